@@ -289,6 +289,13 @@ tb_status tb_op_conv2d(tb_session* session, tb_stream* stream, const tb_tensor* 
 tb_status tb_execute(tb_session* session, tb_stream* stream, const char* op, const tb_tensor* inputs,
                      uint32_t num_inputs, const tb_tensor* output, const tb_attr* attrs, uint32_t num_attrs,
                      tb_event** out);
+/* tb_execute for an OpRequest of any number of outputs: the operators above with one, and
+ * "attention.varlen" (4 or 5 inputs, 1 output), "attention.paged" (6, 1),
+ * "kv_cache.append" (3, 2) and "kv_cache.plan" (3, 5), their tensors in the order of the
+ * tb_op_* entries below. */
+tb_status tb_execute_outputs(tb_session* session, tb_stream* stream, const char* op, const tb_tensor* inputs,
+                             uint32_t num_inputs, const tb_tensor* outputs, uint32_t num_outputs,
+                             const tb_attr* attrs, uint32_t num_attrs, tb_event** out);
 
 /* Runtime::compile (titan-runtime/src/lib.rs:3472-3483) over the Graph IR
  * (titan-graph/src/graph.rs:72-105), shaped like the core pipeline
@@ -374,6 +381,70 @@ tb_status tb_op_gemm_sharded(tb_comm* comm, tb_stream* stream, const tb_tensor* 
 tb_status tb_op_gemm_bias_act(tb_session* session, tb_stream* stream, const tb_tensor* lhs, const tb_tensor* rhs,
                               const tb_tensor* bias, const tb_tensor* output, const tb_attr* attrs,
                               uint32_t num_attrs, tb_event** out);
+
+/* ---------------- Attention over packed and paged sequences ---------------- */
+
+/* No counterpart in the reference. Conventions of the four operators below:
+ *   - BF16 or F16 values (kv_cache.append: F32 too), fp32 scores, softmax statistics and
+ *     accumulation, one rounding of the output; I32 index tensors with contiguous rows.
+ *   - Value tensors may be strided: the innermost dimension contiguous, the others with any
+ *     positive strides (a slice of a fused projection, a cache with heads before rows).
+ *     Outputs' elements may not overlap each other or an input.
+ *   - Query head h uses key head h / (H / Hkv); H is a multiple of Hkv.
+ *   - Lengths, tables and slots are read on the device, so one call (or one captured graph)
+ *     serves steps of different lengths. Values outside the tensors' extents are clamped
+ *     (cu_seqlens, seq_lens), skipped (slots) or read as zero rows (page ids): never followed.
+ *   - With `causal` the mask is aligned at the sequences' ends: query row i of Lq sees the
+ *     keys j <= Lk - Lq + i (tb_op_sdpa aligns at the start; the same when Lq == Lk).
+ *   - A query row that sees no key gives zeros. Query rows behind cu_seqlens_q[batch] are
+ *     left as they were. A key row behind its sequence's end never reaches a result,
+ *     whatever its bits. Inside a sequence a key row with a NaN or an infinity may reach
+ *     rows that the causal mask hides it from.
+ * Attributes of both attention operators: causal (0 or 1), scale (decimal string, > 0,
+ * default 1/sqrt(D)), candidate. D <= 256. */
+
+/* "attention.varlen": Q [Tq, H, D], K/V [Tk, Hkv, D], request b's rows
+ * cu_seqlens[b] .. cu_seqlens[b+1] of them; cu_seqlens [batch + 1], nondecreasing.
+ * cu_seqlens_k NULL: the same as cu_seqlens_q (Tk == Tq). Output [Tq, H, D]. causal
+ * defaults to 0. */
+tb_status tb_op_attention_varlen(tb_session* session, tb_stream* stream, const tb_tensor* q, const tb_tensor* k,
+                                 const tb_tensor* v, const tb_tensor* cu_seqlens_q, const tb_tensor* cu_seqlens_k,
+                                 const tb_tensor* output, const tb_attr* attrs, uint32_t num_attrs, tb_event** out);
+
+/* "attention.paged": new tokens Q [Tq, H, D] over caches [pages, page, Hkv, D]. Key j of
+ * request b is row j % page of page block_table[b, j / page]; seq_lens[b] keys, the new
+ * tokens' own among them (written before by kv_cache.append). block_table [batch, width];
+ * entries past a request's last page are not read. causal defaults to 1. Attribute
+ * max_query_len: no request has more new tokens than this (default: Tq); a step of single
+ * tokens gives 1 and launches less. Rows past the bound may be left as they were. */
+tb_status tb_op_attention_paged(tb_session* session, tb_stream* stream, const tb_tensor* q, const tb_tensor* k_cache,
+                                const tb_tensor* v_cache, const tb_tensor* block_table, const tb_tensor* seq_lens,
+                                const tb_tensor* cu_seqlens_q, const tb_tensor* output, const tb_attr* attrs,
+                                uint32_t num_attrs, tb_event** out);
+
+/* "kv_cache.append": row t of K and V [T, Hkv, D] goes to row slot % page of page
+ * slot / page of the caches, slot = slot_map[t]; a slot outside [0, pages * page) is
+ * skipped. Slots that occur twice leave one of their rows, unspecified which (for
+ * K and V each, and possibly a mixture of their 16-byte pieces). No attributes. */
+tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, const tb_tensor* k, const tb_tensor* v,
+                          const tb_tensor* slot_map, const tb_tensor* k_cache, const tb_tensor* v_cache,
+                          const tb_attr* attrs, uint32_t num_attrs, tb_event** out);
+
+/* "kv_cache.plan": the index tensors of one step, from request lengths. Request b has
+ * context_lens[b] tokens in the cache and adds new_lens[b], packed one request after
+ * another. It holds ceil(context / page_size) pages (the first entries of its block_table
+ * row, which are only read) and takes the ones it lacks from free_pages, in request order.
+ * Writes block_table's new entries, seq_lens = context + new, cu_seqlens (the running sum of
+ * new_lens, [batch + 1]), slot_map (a slot for each packed token, -1 past the last one) and
+ * status = {pages taken from the front of free_pages, requests refused}.
+ * A request is refused when a length is negative, its pages exceed the row, its tokens pass
+ * the end of slot_map, or free_pages ends before its pages (later requests that need pages
+ * are then refused too): its seq_lens is its context, its slots are -1, its row is not
+ * written. Up to 16384 requests. Attribute page_size (required). */
+tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const tb_tensor* context_lens,
+                        const tb_tensor* new_lens, const tb_tensor* free_pages, const tb_tensor* block_table,
+                        const tb_tensor* seq_lens, const tb_tensor* cu_seqlens, const tb_tensor* slot_map,
+                        const tb_tensor* status, const tb_attr* attrs, uint32_t num_attrs, tb_event** out);
 
 /* ---------------- Allocation-free split-K GEMM ---------------- */
 

@@ -150,6 +150,12 @@ _SIGNATURES = {
     "tb_fill_uniform": (_S, [_P, _U32, _SZ, _U64, ctypes.c_double, ctypes.c_double, _S]),
     "tb_execute": (_S, [_P, _P, ctypes.c_char_p, ctypes.POINTER(Tensor), _U32, ctypes.POINTER(Tensor),
                         ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_execute_outputs": (_S, [_P, _P, ctypes.c_char_p, ctypes.POINTER(Tensor), _U32, ctypes.POINTER(Tensor), _U32,
+                                ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_op_attention_varlen": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 6 + [ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_op_attention_paged": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 7 + [ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_op_kv_append": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 5 + [ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_op_kv_plan": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 8 + [ctypes.POINTER(Attr), _U32, _PP]),
     "tb_graph_compile": (_S, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _SZ, ctypes.POINTER(_SZ)]),
     "tb_tune_open": (_S, [ctypes.c_char_p, _PP]),
     "tb_tune_release": (None, [_P]),

@@ -84,6 +84,53 @@ inline tb_status tensor_buffer(Session* s, const tb_tensor* t, const char* what,
   return TB_OK;
 }
 
+// As tensor_buffer for a strided tensor: the innermost dimension contiguous, every other
+// stride positive (a stride of an extent of one is not looked at), all rows inside the buffer.
+inline tb_status strided_buffer(Session* s, const tb_tensor* t, const char* what, Buffer** out) {
+  tb_status rc = check_buffer(s, t->buffer, out);
+  if (rc) return rc;
+  uint64_t last = 0;  // index of the last element
+  const uint64_t room = (*out)->bytes / dtype_size(t->dtype);
+  for (uint32_t a = 0; a < t->rank; ++a) {
+    if (t->shape[a] == 0) return contract(std::string(what) + " requires non-zero dimensions");
+    const uint64_t steps = t->shape[a] - 1;
+    if (steps == 0) continue;
+    if (t->strides[a] < 1 || (a + 1 == t->rank && t->strides[a] != 1))
+      return contract(std::string(what) + " requires a contiguous innermost dimension and positive strides");
+    const unsigned __int128 at = (unsigned __int128)steps * (uint64_t)t->strides[a] + last;
+    if (at >= room) return contract(std::string(what) + " buffer does not hold the tensor's extent");
+    last = (uint64_t)at;
+  }
+  if (room == 0) return contract(std::string(what) + " buffer does not hold the tensor's extent");
+  if ((*out)->ptr % dtype_size(t->dtype) != 0) return contract(std::string(what) + " is not aligned to its elements");
+  return TB_OK;
+}
+
+// Whether no two indices of the tensor name the same element: with the dimensions in order
+// of their strides, each stride passes the extent of the dimensions inside it.
+inline bool distinct_elements(const tb_tensor* t) {
+  uint64_t extent = 1;
+  bool used[TB_MAX_RANK] = {};
+  for (uint32_t n = 0; n < t->rank; ++n) {
+    int inner = -1;
+    for (uint32_t a = 0; a < t->rank; ++a)
+      if (!used[a] && t->shape[a] > 1 && (inner < 0 || t->strides[a] < t->strides[inner])) inner = (int)a;
+    if (inner < 0) break;
+    used[inner] = true;
+    if (t->strides[inner] < 1 || (uint64_t)t->strides[inner] < extent) return false;
+    extent += (uint64_t)t->strides[inner] * (t->shape[inner] - 1);
+  }
+  return true;
+}
+
+// An I32 index tensor: rank 1, or rank 2 with contiguous rows.
+inline bool is_index(const tb_tensor* t, uint32_t rank) {
+  return t->dtype == TB_I32 && t->rank == rank && (t->strides[rank - 1] == 1 || t->shape[rank - 1] <= 1);
+}
+
+// The step of dimension `a` in elements; 0 where the extent is one and the stride is free.
+inline int64_t step_of(const tb_tensor* t, uint32_t a) { return t->shape[a] > 1 ? t->strides[a] : 0; }
+
 // Launches a built-in kernel on a session stream and counts it.
 inline tb_status launch_builtin(Session* s, Stream* st, CUfunction fn, unsigned gx, unsigned gy, unsigned gz,
                                 unsigned bx, unsigned shared_bytes, void** params, const char* candidate,

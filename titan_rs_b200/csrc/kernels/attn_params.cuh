@@ -1,0 +1,77 @@
+// What the packed and paged attention kernels are told about one call: pointers, extents
+// and strides (in elements). Filled by the host entry (op_attention.cpp), passed by value.
+//
+// A request b owns query rows cu_q[b] .. cu_q[b+1] of `q` and `o`, and Lk keys:
+//   packed (table == 0): rows cu_k[b] .. cu_k[b+1] of `k` and `v`;
+//   paged: key j is row j % page of page table[b, j / page], Lk = lens[b].
+// The index tensors live on the device and are not known to the host, so every kernel
+// clamps what it reads from them to the extents given here (request_of below).
+#pragma once
+
+#include <stdint.h>
+
+namespace tb {
+
+struct AttnParams {
+  uint64_t q, k, v, o;     // 16-bit elements
+  uint64_t cu_q, cu_k;     // int32 [batch + 1]; cu_k unused when paged
+  uint64_t table, lens;    // int32 [batch, width], [batch]; 0 when packed
+  int64_t q_tok, q_head;   // strides; the innermost dimension is contiguous everywhere
+  int64_t k_tok, k_head, k_page;
+  int64_t v_tok, v_head, v_page;
+  int64_t o_tok, o_head;
+  int64_t table_row;
+  int32_t tq, tk;          // rows of q; rows of k (packed)
+  int32_t batch, heads, kv_heads, dim;
+  int32_t page, pages, width;
+  int32_t causal;
+  float scale;             // factor of q . k
+};
+
+// The index arithmetic is shared by the kernels and a host test of it.
+#ifdef __CUDACC__
+#define TB_INDEX_FN __device__ __forceinline__
+TB_INDEX_FN int load_index(const int* p) { return __ldg(p); }
+#else
+#define TB_INDEX_FN inline
+TB_INDEX_FN int load_index(const int* p) { return *p; }
+#endif
+
+// Request b: its query rows [q0, q0 + lq) and its keys (lk of them, from row k0 when packed).
+struct AttnRequest {
+  int q0, lq, k0, lk;
+};
+
+TB_INDEX_FN int clamp_index(int64_t x, int64_t lo, int64_t hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
+
+TB_INDEX_FN AttnRequest request_of(const AttnParams& p, int b) {
+  const int* cu_q = reinterpret_cast<const int*>(p.cu_q);
+  AttnRequest r;
+  r.q0 = clamp_index(load_index(cu_q + b), 0, p.tq);
+  r.lq = clamp_index(load_index(cu_q + b + 1), r.q0, p.tq) - r.q0;
+  if (p.table) {
+    const int64_t most = (int64_t)p.width * p.page;
+    r.k0 = 0;
+    r.lk = clamp_index(load_index(reinterpret_cast<const int*>(p.lens) + b), 0, most);
+  } else {
+    const int* cu_k = reinterpret_cast<const int*>(p.cu_k);
+    r.k0 = clamp_index(load_index(cu_k + b), 0, p.tk);
+    r.lk = clamp_index(load_index(cu_k + b + 1), r.k0, p.tk) - r.k0;
+  }
+  return r;
+}
+
+// Leading keys that query row i of the request sees. The causal mask is aligned at the
+// ends: the last query row sees every key.
+TB_INDEX_FN int visible_keys(const AttnParams& p, const AttnRequest& r, int i) {
+  return p.causal ? clamp_index((int64_t)r.lk - r.lq + i + 1, 0, r.lk) : r.lk;
+}
+
+// Page `index` of request b, or -1 when the table names none of the cache's pages (its keys
+// read as zeros).
+TB_INDEX_FN int page_of(const AttnParams& p, int b, int index) {
+  const int id = load_index(reinterpret_cast<const int*>(p.table) + b * p.table_row + index);
+  return id >= 0 && id < p.pages ? id : -1;
+}
+
+}  // namespace tb

@@ -1,5 +1,6 @@
 """Operator entry: the titan.rs `Runtime::execute(OpRequest)` path for the four
-hot-path operators, dispatched to libtitan_b200's tb_op_* entry points.
+hot-path operators and the serving operators (attention over packed and paged sequences,
+the cache's plan and append), dispatched to libtitan_b200's tb_op_* entry points.
 
 Mirrors projects/titan-runtime/src/lib.rs:1171-1256 (dispatch by operator name
 when the first input lives on the CUDA backend), TensorHandle/TensorSpec
@@ -172,15 +173,26 @@ def _attrs(attrs: dict):
 
 
 _OPS = {"softmax": "tb_op_softmax", "gemm": "tb_op_gemm", "scaled_dot_product_attention": "tb_op_sdpa",
-        "conv2d": "tb_op_conv2d", "gemm.bias_act": "tb_op_gemm_bias_act", "attention.fused": "tb_op_sdpa"}
+        "conv2d": "tb_op_conv2d", "gemm.bias_act": "tb_op_gemm_bias_act", "attention.fused": "tb_op_sdpa",
+        "attention.varlen": "tb_op_attention_varlen", "attention.paged": "tb_op_attention_paged",
+        "kv_cache.append": "tb_op_kv_append", "kv_cache.plan": "tb_op_kv_plan"}
 _ARITY = {"softmax": (1, 1), "gemm": (2, 2), "scaled_dot_product_attention": (3, 3), "conv2d": (2, 3),
-          "gemm.bias_act": (2, 3), "attention.fused": (3, 3)}
+          "gemm.bias_act": (2, 3), "attention.fused": (3, 3), "attention.varlen": (4, 5), "attention.paged": (6, 6),
+          "kv_cache.append": (3, 3), "kv_cache.plan": (3, 3)}
+# Operators with several outputs. They write into tensors that already hold something (the
+# caches, the block table), so the caller passes these.
+_OUTPUTS = {"kv_cache.append": 2, "kv_cache.plan": 5}
 _ARITY_MSG = {"softmax": "CUDA softmax requires exactly one input and one output",
               "gemm": "gemm requires exactly two rank-2 inputs",
               "scaled_dot_product_attention": "scaled dot-product attention requires exactly three rank-4 BHTD inputs",
               "conv2d": "conv2d requires rank-4 NCHW input, rank-4 OIHW weight, and optional bias",
               "gemm.bias_act": "gemm.bias_act requires two rank-2 inputs, an optional bias and one output",
-              "attention.fused": "attention.fused requires Q, K and V"}
+              "attention.fused": "attention.fused requires Q, K and V",
+              "attention.varlen": "attention.varlen requires Q, K, V, cu_seqlens_q and an optional cu_seqlens_k",
+              "attention.paged": "attention.paged requires Q, K cache, V cache, block_table, seq_lens and cu_seqlens_q",
+              "kv_cache.append": "kv_cache.append requires K, V and slot_map, and the K and V caches as outputs",
+              "kv_cache.plan": "kv_cache.plan requires context_lens, new_lens and free_pages, and the outputs "
+                               "block_table, seq_lens, cu_seqlens, slot_map and status"}
 
 
 class Runtime:
@@ -201,45 +213,70 @@ class Runtime:
         self._device_key = None
         self._artifact = None
 
-    def execute(self, request: OpRequest, output: Optional[TensorHandle] = None) -> ExecutionHandle:
+    def execute(self, request: OpRequest, output=None) -> ExecutionHandle:
+        """Enqueues a request. `output`: the tensor to write, or the list of them for an operator
+        of several outputs; one output may be left out and is then allocated."""
+        name = request.operator
+        outputs = self._checked(request, output)
+        attrs = dict(request.attrs)
+        self.last_tune = None
+        if self.autotuner is not None and "candidate" not in attrs and len(outputs) == 1:
+            chosen = self._tuned_candidate(request, outputs[0], attrs)
+            if chosen:
+                attrs["candidate"] = chosen
+        ev = self._launch(name, request, outputs, attrs)
+        L = N.lib()
+        return ExecutionHandle(self._result(request, outputs), L.tb_last_candidate().decode(),
+                               L.tb_last_candidate().decode(), Event(self.session, ev))
+
+    def bind(self, request: OpRequest, output=None) -> "BoundRequest":
+        """A request that is enqueued many times over the same tensors (a serving step): its
+        arguments cross the ABI once, and each BoundRequest.enqueue() is one native call."""
+        return BoundRequest(self, request, self._checked(request, output))
+
+    def _checked(self, request: OpRequest, output) -> list:
+        """The request's checks on this side of the ABI, and its output tensors."""
         name = request.operator
         if name not in _OPS:
             raise ExecutionError(name, "contract", f"operator {name} is not on the B200 hot path (does not implement)",
                                  N.TB_ERR_UNSUPPORTED)
         lo, hi = _ARITY[name]
-        if not (lo <= len(request.inputs) <= hi) or len(request.outputs) != 1:
+        if not (lo <= len(request.inputs) <= hi) or len(request.outputs) != _OUTPUTS.get(name, 1):
             raise ExecutionError(name, "contract", _ARITY_MSG[name])
         for t in request.inputs:
             if t.session is not self.session:
                 raise ExecutionError(name, "contract", f"CUDA {name} requires inputs from the same session")
-        spec = request.outputs[0]
-        if output is None:
+        if output is None and name not in _OUTPUTS:
+            spec = request.outputs[0]
             try:
-                output = TensorHandle.allocate(self.session, spec.dtype, spec.shape)
+                return [TensorHandle.allocate(self.session, spec.dtype, spec.shape)]
             except HalError as e:
                 raise ExecutionError(name, "allocate", str(e), e.status) from e
-        attrs = dict(request.attrs)
-        self.last_tune = None
-        if self.autotuner is not None and "candidate" not in attrs:
-            chosen = self._tuned_candidate(request, output, attrs)
-            if chosen:
-                attrs["candidate"] = chosen
-        ev = self._launch(name, request, output, attrs)
-        L = N.lib()
-        return ExecutionHandle([TensorHandle(self.session, output.buffer, spec.dtype, tuple(spec.shape),
-                                             contiguous_strides(spec.shape))],
-                               L.tb_last_candidate().decode(), L.tb_last_candidate().decode(),
-                               Event(self.session, ev))
+        outputs = list(output) if isinstance(output, (list, tuple)) else [] if output is None else [output]
+        if len(outputs) != len(request.outputs):
+            raise ExecutionError(name, "contract", f"{name} writes into existing tensors: pass "
+                                                   f"output=[{len(request.outputs)} tensors]")
+        return outputs
 
-    def _launch(self, name: str, request: OpRequest, output: TensorHandle, attrs_dict: dict) -> int:
-        """One request through tb_execute, the native Runtime::execute router."""
-        spec = request.outputs[0]
-        out_c = c_tensor(output.buffer, spec.dtype, spec.shape, spec.resolved_strides())
+    def _result(self, request: OpRequest, outputs: list) -> list:
+        return [TensorHandle(self.session, t.buffer, spec.dtype, tuple(spec.shape),
+                             spec.resolved_strides() if spec.strides is not None else contiguous_strides(spec.shape))
+                for t, spec in zip(outputs, request.outputs)]
+
+    def _arguments(self, name: str, request: OpRequest, outputs: list, attrs_dict: dict) -> tuple:
+        """The arguments of tb_execute_outputs up to the event, and what must outlive the call."""
+        outs = (N.Tensor * len(outputs))(*[c_tensor(t.buffer, spec.dtype, spec.shape, spec.resolved_strides())
+                                           for t, spec in zip(outputs, request.outputs)])
         ins = (N.Tensor * len(request.inputs))(*[t.c_tensor() for t in request.inputs])
-        attrs, nattrs, _keep = _attrs(attrs_dict)
+        attrs, nattrs, keep = _attrs(attrs_dict)
+        return (self.session.ptr, self.stream.ptr, name.encode(), ins, len(request.inputs), outs, len(outputs), attrs,
+                nattrs), keep
+
+    def _launch(self, name: str, request: OpRequest, outputs: list, attrs_dict: dict) -> int:
+        """One request through tb_execute_outputs, the native Runtime::execute router."""
+        args, _keep = self._arguments(name, request, outputs, attrs_dict)
         ev = ctypes.c_void_p(0)
-        st = N.lib().tb_execute(self.session.ptr, self.stream.ptr, name.encode(), ins, len(request.inputs),
-                                ctypes.byref(out_c), attrs, nattrs, ctypes.byref(ev))
+        st = N.lib().tb_execute_outputs(*args, ctypes.byref(ev))
         if st != N.TB_OK:
             op, detail = N.last_error()
             raise ExecutionError(name, op or "launch", detail, st)
@@ -276,7 +313,7 @@ class Runtime:
 
         def run(c):
             try:
-                self._launch(name, request, output, {**attrs, "candidate": c})
+                self._launch(name, request, [output], {**attrs, "candidate": c})
                 self.session.synchronize(self.stream)
             except ExecutionError as e:
                 if e.status == N.TB_ERR_UNSUPPORTED:
@@ -290,10 +327,10 @@ class Runtime:
         def time_ns(c, warmups, samples):
             cand_attrs = {**attrs, "candidate": c}
             for _ in range(warmups):
-                self._launch(name, request, output, cand_attrs)
+                self._launch(name, request, [output], cand_attrs)
             marks = [self.session.record(self.stream)]
             for _ in range(samples):
-                self._launch(name, request, output, cand_attrs)
+                self._launch(name, request, [output], cand_attrs)
                 marks.append(self.session.record(self.stream))
             self.session.synchronize(self.stream)
             return [self.session.elapsed_ms(marks[i], marks[i + 1]) * 1e6 for i in range(samples)]
@@ -304,6 +341,36 @@ class Runtime:
         self.autotuner.flush()
         self.last_tune = result
         return result.entry.candidate
+
+
+class BoundRequest:
+    """A request over fixed tensors (Runtime.bind): enqueue() launches it on the runtime's stream
+    with one native call and no event. It holds the tensors' buffers until it is dropped."""
+
+    def __init__(self, runtime: Runtime, request: OpRequest, outputs: list):
+        self.runtime = runtime
+        self.outputs = runtime._result(request, outputs)
+        self._name = request.operator
+        self._args, self._keep = runtime._arguments(request.operator, request, outputs, dict(request.attrs))
+        self._session, self._stream = runtime.session, runtime.stream
+        self._call = N.lib().tb_execute_outputs
+        self._buffers = [t.buffer for t in [*request.inputs, *outputs]]
+        self._held = [b.ptr for b in self._buffers]
+        for ptr in self._held:
+            N.lib().tb_buffer_retain(ptr)
+
+    def enqueue(self) -> None:
+        if self._session.ptr != self._args[0] or self._stream.ptr != self._args[1]:
+            raise ExecutionError(self._name, "contract", "the request's session or stream was released")
+        st = self._call(*self._args, None)
+        if st != N.TB_OK:
+            op, detail = N.last_error()
+            raise ExecutionError(self._name, op or "launch", detail, st)
+
+    def __del__(self):
+        held, self._held = getattr(self, "_held", []), []
+        for ptr in held:
+            N.lib().tb_buffer_release(ptr)
 
 
 def fill_normal(count: int, seed: int, mean: float = 0.0, std: float = 1.0, dtype: DType = DType.F32,
