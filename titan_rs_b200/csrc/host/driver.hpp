@@ -20,6 +20,7 @@ namespace tb {
   X(cuDevicePrimaryCtxRelease_v2)      \
   X(cuCtxSetCurrent)                   \
   X(cuCtxGetCurrent)                   \
+  X(cuCtxSynchronize)                  \
   X(cuMemAlloc_v2)                     \
   X(cuMemFree_v2)                      \
   X(cuMemGetInfo_v2)                   \
@@ -38,6 +39,8 @@ namespace tb {
   X(cuStreamBeginCapture_v2)           \
   X(cuStreamIsCapturing)               \
   X(cuStreamEndCapture)                \
+  X(cuStreamGetCaptureInfo_v2)         \
+  X(cuThreadExchangeStreamCaptureMode) \
   X(cuGraphInstantiateWithFlags)       \
   X(cuGraphLaunch)                     \
   X(cuGraphExecDestroy)                \

@@ -10,6 +10,8 @@
 // the capture and tb_capture_end reports it: host-staged uploads and downloads (their
 // host side runs at enqueue time), waits on the host, and an operator's first use of
 // per-stream scratch memory (it allocates), so such an operator runs once before capture.
+// The attention operators' workspace is the graph's own (stream_workspace): allocated at
+// capture, freed with the graph, shared with no other graph and no eager call.
 // A replay reads and writes the same device buffers the captured work named.
 #include "internal.hpp"
 
@@ -18,6 +20,7 @@ namespace tb {
 struct GraphExec : RefCounted {
   Session* session = nullptr;
   CUgraphExec exec = nullptr;
+  std::vector<CUdeviceptr> work;  // workspace of its operators (stream_workspace)
 };
 
 }  // namespace tb
@@ -49,17 +52,28 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
   if (rc) return rc;
   const DriverApi* d = driver();
   CUgraph graph = nullptr;
+  const unsigned long long id = capture_id(st);
+  std::vector<CUdeviceptr> work = id ? take_captured_work(s, id) : std::vector<CUdeviceptr>();
+  const auto drop_work = [&] {
+    for (CUdeviceptr p : work) d->cuMemFree_v2(p);
+  };
   // Ends the capture in every case; an invalidated capture (a call that cannot be
   // captured ran meanwhile) reports the driver's error and yields no graph.
-  TB_CU("cuStreamEndCapture", d->cuStreamEndCapture(st->raw, &graph));
+  const CUresult ended = d->cuStreamEndCapture(st->raw, &graph);
+  if (ended != CUDA_SUCCESS || !graph) drop_work();
+  if (ended != CUDA_SUCCESS) return cu_error("cuStreamEndCapture", ended);
   if (!graph) return set_error(TB_ERR_INVALID, "capture", "nothing was captured");
   CUgraphExec exec = nullptr;
   const CUresult r = d->cuGraphInstantiateWithFlags(&exec, graph, 0);
   d->cuGraphDestroy(graph);
-  if (r != CUDA_SUCCESS) return cu_error("cuGraphInstantiate", r);
+  if (r != CUDA_SUCCESS) {
+    drop_work();
+    return cu_error("cuGraphInstantiate", r);
+  }
   GraphExec* g = new GraphExec();
   g->session = s;
   g->exec = exec;
+  g->work = std::move(work);
   s->refs.fetch_add(1);
   *out = reinterpret_cast<tb_graph_exec*>(g);
   return TB_OK;
@@ -87,6 +101,8 @@ void tb_graph_exec_release(tb_graph_exec* graph) {
   if (d && g->exec) {
     d->cuCtxSetCurrent(s->context);
     d->cuGraphExecDestroy(g->exec);  // a replay still in flight completes; the driver frees it then
+    if (!g->work.empty()) d->cuCtxSynchronize();  // and may still use its workspace
+    for (CUdeviceptr p : g->work) d->cuMemFree_v2(p);
   }
   delete g;
   tb_session_release(reinterpret_cast<tb_session*>(s));

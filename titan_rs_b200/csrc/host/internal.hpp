@@ -52,6 +52,21 @@ struct Stream : RefCounted {
   // Stream order serialises its users; it grows on demand and is freed with the stream.
   CUdeviceptr scratch = 0;
   size_t scratch_bytes = 0;
+  // Workspace of the attention operators (zeroed when allocated, and left with its counters
+  // at zero by every launch). `enqueue` is held while an operator takes it and launches, so
+  // that a second host thread on the stream cannot replace it in between.
+  CUdeviceptr work = 0;
+  size_t work_bytes = 0;
+  std::mutex enqueue;
+};
+
+// Workspace that operators took while their stream was being captured: it belongs to the
+// graph (two graphs, or a graph and eager calls, never share one).
+struct CapturedWork {
+  unsigned long long capture;  // the driver's id of the capture
+  Stream* stream;
+  CUdeviceptr ptr;
+  size_t bytes;
 };
 
 struct Event : RefCounted {
@@ -97,6 +112,7 @@ struct Session : RefCounted {
   std::unordered_map<std::string, std::shared_ptr<Module>> builtin_modules;
   std::unordered_map<CUfunction, int> pair_occupancy;  // resident CTA pairs of a built-in pair kernel
   std::unordered_set<void*> pinned;
+  std::vector<CapturedWork> captured_work;  // of captures that have not ended
   StatusWord status;
   int sm_count = 0;
   int max_smem_optin = 0;
@@ -113,6 +129,14 @@ tb_status check_event(Session* s, tb_event* e, Event** out);
 
 // At least `bytes` of the stream's scratch memory (allocating or growing it).
 tb_status stream_scratch(Session* s, Stream* st, size_t bytes, CUdeviceptr* out);
+
+// At least `bytes` of zeroed-at-first workspace for an operator on the stream: the stream's
+// own, or, while the stream is being captured, memory of the graph. The caller holds st->enqueue.
+tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* out);
+// The id of the capture that `st` is part of, 0 outside a capture.
+unsigned long long capture_id(Stream* st);
+// Takes the workspaces of an ended capture out of the session's list.
+std::vector<CUdeviceptr> take_captured_work(Session* s, unsigned long long capture);
 
 // Whether `st` is being captured into a CUDA graph (tb_capture_begin): host-staged
 // copies and allocations are refused then, since a replay would run them on memory

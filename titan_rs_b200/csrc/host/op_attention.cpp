@@ -2,6 +2,7 @@
 // lengths, with grouped key heads, over contiguous K and V or over a paged cache. No
 // counterpart in the reference, whose attention takes one [B, H, T, D] block
 // (titan-runtime/src/lib.rs:1090-1151); the checks and messages follow its manner.
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 
@@ -92,6 +93,30 @@ tb_status launch_rows(Session* s, Stream* st, AttnCall* c) {
   return launch_builtin(s, st, fn, (unsigned)grid, 1, 1, 256, 0, params, entry);
 }
 
+// Whether the tensor cores' 16-byte copies reach every row of K and V, and 4-byte loads every
+// row of Q.
+bool rows_aligned(const AttnParams& p) {
+  const uint64_t kv = p.k | p.v | (uint64_t)(2 * (p.k_tok | p.k_head | p.k_page | p.v_tok | p.v_head | p.v_page));
+  const uint64_t q = p.q | (uint64_t)(2 * (p.q_tok | p.q_head));
+  return (p.dim == 64 || p.dim == 128) && (kv & 15) == 0 && (q & 3) == 0;
+}
+
+// Decode kernel for the requests of at most p.token_rows (row, head) pairs per key head.
+tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
+  const std::string entry = std::string("attention_tokens_") + (c->dtype == TB_BF16 ? "bf16" : "f16") + "_d" +
+                            std::to_string(c->p.dim) + "_r" + std::to_string(c->p.token_rows);
+  CUfunction fn = nullptr;
+  tb_status rc = builtin_function(s, "attn_tokens", entry.c_str(), &fn);
+  if (rc) return rc;
+  const int ctas = std::min(2 * s->sm_count, kTokenCounters);  // two resident on each SM
+  CUdeviceptr work = 0;
+  if ((rc = stream_workspace(s, st, token_workspace_bytes(ctas, c->p.token_rows, c->p.dim), &work))) return rc;
+  c->p.work = work;
+  void* params[] = {&c->p};
+  return launch_builtin(s, st, fn, (unsigned)ctas, 1, 1, kTokenThreads, (unsigned)token_smem_bytes(c->p.dim), params,
+                        entry.c_str());
+}
+
 tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, const AttnAttrs& a) {
   tb_status rc = activate(s);
   if (rc) return rc;
@@ -99,6 +124,15 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
   c->p.scale = (float)(a.scale > 0.0 ? a.scale : 1.0 / std::sqrt((double)c->p.dim));
   if (a.candidate && strcmp(a.candidate, "attention_rows") != 0)
     return contract(std::string("unknown ") + op + " candidate " + a.candidate);
+  std::lock_guard<std::mutex> lock(st->enqueue);
+  const uint64_t group = (uint64_t)(c->p.heads / c->p.kv_heads);
+  const uint64_t longest = a.max_query && a.max_query < (uint64_t)c->p.tq ? a.max_query : (uint64_t)c->p.tq;
+  if (c->p.table && !a.candidate && rows_aligned(c->p) && group <= 32) {
+    // Sized for every request where the caller's bound says so, for single tokens otherwise.
+    const uint64_t rows = longest * group <= 32 ? longest * group : group;
+    c->p.token_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    if ((rc = launch_tokens(s, st, c)) || longest * group <= (uint64_t)c->p.token_rows) return rc;
+  }
   return launch_rows(s, st, c);
 }
 

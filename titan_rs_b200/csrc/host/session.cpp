@@ -176,6 +176,7 @@ void session_destroy(Session* s) {
     if (d && st->raw) {
       d->cuStreamSynchronize(st->raw);
       if (st->scratch) d->cuMemFree_v2(st->scratch);
+      if (st->work) d->cuMemFree_v2(st->work);
       d->cuStreamDestroy_v2(st->raw);
     }
     delete st;
@@ -184,6 +185,8 @@ void session_destroy(Session* s) {
     if (d && b->owned && b->ptr) d->cuMemFree_v2(b->ptr);
     delete b;
   }
+  for (const CapturedWork& w : s->captured_work)
+    if (d) d->cuMemFree_v2(w.ptr);
   for (void* p : s->pinned)
     if (d) d->cuMemFreeHost(p);
   if (d && s->status.host) d->cuMemFreeHost((void*)s->status.host);
@@ -289,6 +292,84 @@ tb_status stream_scratch(Session* s, Stream* st, size_t bytes, CUdeviceptr* out)
   st->scratch_bytes = bytes;
   (void)s;
   *out = p;
+  return TB_OK;
+}
+
+unsigned long long capture_id(Stream* st) {
+  CUstreamCaptureStatus status = CU_STREAM_CAPTURE_STATUS_NONE;
+  cuuint64_t id = 0;
+  if (driver()->cuStreamGetCaptureInfo_v2(st->raw, &status, &id, nullptr, nullptr, nullptr) != CUDA_SUCCESS ||
+      status == CU_STREAM_CAPTURE_STATUS_NONE)
+    return 0;
+  return id;
+}
+
+std::vector<CUdeviceptr> take_captured_work(Session* s, unsigned long long capture) {
+  std::vector<CUdeviceptr> got;
+  std::lock_guard<std::mutex> lock(s->mu);
+  std::vector<CapturedWork> kept;
+  for (const CapturedWork& w : s->captured_work) {
+    if (w.capture == capture) got.push_back(w.ptr);
+    else kept.push_back(w);
+  }
+  s->captured_work.swap(kept);
+  return got;
+}
+
+namespace {
+
+// Zeroed device memory, also while a stream of this thread is being captured (the calls
+// here touch no capturing stream, so the capture is not asked to record them).
+tb_status zeroed_memory(size_t bytes, CUdeviceptr* out) {
+  const DriverApi* d = driver();
+  CUstreamCaptureMode mode = CU_STREAM_CAPTURE_MODE_RELAXED;
+  TB_CU("cuThreadExchangeStreamCaptureMode", d->cuThreadExchangeStreamCaptureMode(&mode));
+  CUdeviceptr p = 0;
+  CUstream side = nullptr;
+  CUresult r = d->cuMemAlloc_v2(&p, bytes);
+  if (r == CUDA_SUCCESS) r = d->cuStreamCreate(&side, CU_STREAM_NON_BLOCKING);
+  if (r == CUDA_SUCCESS) r = d->cuMemsetD8Async(p, 0, bytes, side);
+  if (r == CUDA_SUCCESS) r = d->cuStreamSynchronize(side);
+  if (side) d->cuStreamDestroy_v2(side);
+  if (r != CUDA_SUCCESS && p) d->cuMemFree_v2(p);
+  d->cuThreadExchangeStreamCaptureMode(&mode);
+  if (r != CUDA_SUCCESS) return cu_error("allocate", r);
+  *out = p;
+  return TB_OK;
+}
+
+}  // namespace
+
+tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* out) {
+  if (const unsigned long long id = capture_id(st)) {
+    {
+      std::lock_guard<std::mutex> lock(s->mu);
+      for (const CapturedWork& w : s->captured_work)
+        if (w.capture == id && w.stream == st && w.bytes >= bytes) {
+          *out = w.ptr;
+          return TB_OK;
+        }
+    }
+    tb_status rc = zeroed_memory(bytes, out);
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lock(s->mu);
+    s->captured_work.push_back({id, st, *out, bytes});
+    return TB_OK;
+  }
+  if (st->work_bytes < bytes) {
+    const DriverApi* d = driver();
+    if (st->work) {
+      // Earlier kernels on this stream may still use the old one.
+      TB_CU("cuStreamSynchronize", d->cuStreamSynchronize(st->raw));
+      d->cuMemFree_v2(st->work);
+      st->work = 0;
+      st->work_bytes = 0;
+    }
+    tb_status rc = zeroed_memory(bytes, &st->work);
+    if (rc) return rc;
+    st->work_bytes = bytes;
+  }
+  *out = st->work;
   return TB_OK;
 }
 
@@ -514,9 +595,10 @@ void tb_stream_release(tb_stream* stream) {
   const DriverApi* d = driver();
   if (d && x->raw) {
     d->cuCtxSetCurrent(s->context);
-    if (x->scratch) {
+    if (x->scratch || x->work) {
       d->cuStreamSynchronize(x->raw);
-      d->cuMemFree_v2(x->scratch);
+      if (x->scratch) d->cuMemFree_v2(x->scratch);
+      if (x->work) d->cuMemFree_v2(x->work);
     }
     d->cuStreamDestroy_v2(x->raw);
   }

@@ -10,6 +10,12 @@
 
 #include <stdint.h>
 
+#ifdef __CUDACC__
+#define TB_BOTH __host__ __device__
+#else
+#define TB_BOTH
+#endif
+
 namespace tb {
 
 struct AttnParams {
@@ -25,8 +31,28 @@ struct AttnParams {
   int32_t batch, heads, kv_heads, dim;
   int32_t page, pages, width;
   int32_t causal;
+  int32_t token_rows;      // requests of at most this many (query row, head) pairs per key head
+                           // belong to the token kernel, the others to the kernel beside it
   float scale;             // factor of q . k
+  uint64_t work;           // the token kernel's workspace: counters, then partial results
 };
+
+// Layout of the token kernel's workspace: a counter per CTA, at the same place for every form
+// of the kernel (it is zero between launches), then two partial results a CTA (its first
+// request may have begun in an earlier CTA, its last may go on in a later one), each
+// rows x (dim + 2) floats: O, then the row's maximum and sum.
+constexpr int kTokenCounters = 1024;  // CTAs at most
+TB_BOTH constexpr uint64_t token_slot_floats(int rows, int dim) { return (uint64_t)rows * (dim + 2); }
+TB_BOTH constexpr uint64_t token_workspace_bytes(int ctas, int rows, int dim) {
+  return 4ull * kTokenCounters + 2ull * ctas * token_slot_floats(rows, dim) * 4;
+}
+
+// The token kernel: keys of a tile, stages of its ring, and its shared memory (the ring, the
+// row offsets of two tiles, the joined statistics and some words; 128 bytes to align).
+constexpr int kTokenTile = 64, kTokenStages = 3, kTokenThreads = 128;
+TB_BOTH constexpr int token_smem_bytes(int dim) {
+  return kTokenStages * 2 * kTokenTile * dim * 2 + 2 * kTokenTile * 16 + 2 * 4 * 8 * 4 + 128 + 128;
+}
 
 // The index arithmetic is shared by the kernels and a host test of it.
 #ifdef __CUDACC__
@@ -59,6 +85,11 @@ TB_INDEX_FN AttnRequest request_of(const AttnParams& p, int b) {
     r.lk = clamp_index(load_index(cu_k + b + 1), r.k0, p.tk) - r.k0;
   }
   return r;
+}
+
+// Whether the request is the token kernel's (it has query rows, and few enough).
+TB_INDEX_FN bool is_token_request(const AttnParams& p, const AttnRequest& r) {
+  return r.lq > 0 && (int64_t)r.lq * (p.heads / p.kv_heads) <= p.token_rows;
 }
 
 // Leading keys that query row i of the request sees. The causal mask is aligned at the

@@ -40,7 +40,7 @@ __device__ __forceinline__ void attention_rows(const AttnParams& p) {
     if (lo == 0) continue;
     const int b = lo - 1;
     const AttnRequest r = request_of(p, b);
-    if (t < r.q0 || t >= r.q0 + r.lq) continue;
+    if (t < r.q0 || t >= r.q0 + r.lq || is_token_request(p, r)) continue;
     const int n = visible_keys(p, r, t - r.q0);
     const int hk = h / (p.heads / p.kv_heads);
     const T* q = reinterpret_cast<const T*>(p.q) + t * p.q_tok + h * p.q_head;

@@ -1,0 +1,468 @@
+// Attention of a few query rows per request over a long paged cache: the decode step.
+//
+//   O = sum_j 2^(c s_j - m) v_j / sum_j 2^(c s_j - m),  s_j = q . k_j,  c = scale log2(e)
+//
+// Every cached row is read once for the G x Lq (query row, head) pairs of its key head, so at
+// 2 G Lq flops a byte the kernel is bound by the HBM, and the design serves the loads:
+//   - One list of 64-key tiles over all (request, key head) pairs is cut into equal runs, one
+//     per CTA (two CTAs an SM), so requests of any lengths load the SMs evenly. A pair that
+//     is cut leaves partial results (O, m, sum) in the workspace; the CTA that finishes it
+//     last adds them up in the order of the runs, so the result does not depend on who is last.
+//   - Tiles arrive in a ring of shared-memory stages by 16-byte cp.async, which takes any
+//     page size and cache layout, and fills rows past the sequence's end (and of page ids
+//     that name no page) with zeros: their bits never reach a product. Page ids are read
+//     one tile ahead of the copies that need them.
+//   - The products run as S^T = K Q^T and O^T = V^T P^T on m16n8k16 tensor-core
+//     instructions: keys and dimensions fill the 16 rows, the few query rows the 8
+//     columns (a tcgen05 tile has 64 or 128 rows, of which a decode step would fill 8). Each
+//     warp takes 16 keys of a tile with a maximum and sum of its own, so the warps
+//     meet only for the stage hand-over; they are joined when the pair ends.
+// Scores, statistics and O are fp32; P is rounded to the values' type for the second product
+// (at most 2^8: the reference maximum moves only when a row's maximum grows by more than 2^8).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "attn_math.cuh"
+#include "attn_params.cuh"
+
+namespace {
+
+using namespace tb;
+
+constexpr int kTile = kTokenTile;  // 16 keys a warp
+constexpr int kThreads = kTokenThreads;
+constexpr int kStages = kTokenStages;
+constexpr float kLowest = -3.402823466e38f;
+
+template <int D>
+TB_BOTH constexpr int stage_bytes() { return 2 * kTile * D * 2; }
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes to shared memory without a register, or 16 zero bytes.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void load_matrix(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_matrix_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+};
+template <>
+struct Half<__half> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+};
+
+// Tiles of one (request, key head) pair; 0 for a request that is not this kernel's. A
+// request without keys has one empty tile, which writes its zeros.
+__device__ __forceinline__ int tiles_of(const AttnParams& p, const AttnRequest& r) {
+  return is_token_request(p, r) ? max(1, (r.lk + kTile - 1) / kTile) : 0;
+}
+
+// A position in the list of tiles: request-major, then key heads, then tiles.
+struct Cursor {
+  int b, head, tile, tiles;
+  AttnRequest r;
+
+  // To request `from` or the first one behind it that has tiles.
+  __device__ __forceinline__ void seek(const AttnParams& p, int from) {
+    head = tile = 0;
+    tiles = 0;
+    for (b = from; b < p.batch; ++b) {
+      r = request_of(p, b);
+      tiles = tiles_of(p, r);
+      if (tiles) break;
+    }
+  }
+  __device__ __forceinline__ void next(const AttnParams& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++head < p.kv_heads) return;
+    seek(p, b + 1);
+  }
+};
+
+template <int D>
+struct Shared {
+  alignas(128) uint8_t stage[kStages][stage_bytes<D>()];  // K rows, then V rows; 16-byte chunks swizzled by row
+  long long k_at[2][kTile], v_at[2][kTile];  // element offsets of a tile's rows, or -1
+  float top[4][8], sum[4][8];
+  long long scan[kThreads / 32], found_before;
+  int found_b, last;
+};
+
+template <typename T, int D, int NT>
+__device__ __forceinline__ void attention_tokens(const AttnParams& p) {
+  extern __shared__ uint8_t raw[];
+  Shared<D>& sm = *reinterpret_cast<Shared<D>*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
+  constexpr int kRows = 8 * NT;
+  constexpr int kChunks = D / 8;                    // 16-byte chunks of a row
+  constexpr int kRowsAtOnce = kThreads / kChunks;   // rows one pass of the CTA copies
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = p.heads / p.kv_heads;
+
+  // ---- this CTA's run of tiles: every thread adds up a stretch of requests ----
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int lo = min(tid * per, p.batch), hi = min(lo + per, p.batch);
+  long long mine = 0;
+  for (int b = lo; b < hi; ++b) mine += tiles_of(p, request_of(p, b));
+  long long upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += x;
+  }
+  if (lane == 31) sm.scan[warp] = upto;
+  __syncthreads();
+  long long before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sm.scan[w];
+    total += sm.scan[w];
+  }
+  total *= p.kv_heads;
+  const long long ctas = min((long long)gridDim.x, total);
+  if (blockIdx.x >= ctas) return;
+  const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
+  {
+    // The request that holds tile `begin`: its requests' tiles start at kv_heads x (tiles before).
+    long long at = before;
+    for (int b = lo; b < hi; ++b) {
+      const int n = tiles_of(p, request_of(p, b));
+      if (at * p.kv_heads <= begin && begin < (at + n) * p.kv_heads) {
+        sm.found_b = b;
+        sm.found_before = at;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  Cursor cur;
+  cur.seek(p, sm.found_b);
+  {
+    const long long inside = begin - sm.found_before * p.kv_heads;
+    cur.head = (int)(inside / cur.tiles);
+    cur.tile = (int)(inside % cur.tiles);
+  }
+  Cursor ahead = cur;  // of the next tile whose rows are looked up
+  const int count = (int)(end - begin);
+
+  // Row offsets of tile `ahead`, by the first kTile threads.
+  auto look_up = [&](long long& k_off, long long& v_off) {
+    const int j = ahead.tile * kTile + tid;
+    k_off = v_off = -1;
+    if (j < ahead.r.lk) {
+      const int id = page_of(p, ahead.b, j / p.page);
+      if (id >= 0) {
+        const int row = j % p.page;
+        k_off = id * p.k_page + row * p.k_tok + ahead.head * p.k_head;
+        v_off = id * p.v_page + row * p.v_tok + ahead.head * p.v_head;
+      }
+    }
+  };
+  // Copies of tile n (its offsets are in shared memory) into its stage.
+  const int chunk = tid % kChunks, row0 = tid / kChunks;
+  auto copy_tile = [&](int n) {
+    const uint32_t base = smem_of(sm.stage[n % kStages]);
+#pragma unroll
+    for (int r = row0; r < kTile; r += kRowsAtOnce) {
+      const uint32_t at = base + r * (D * 2) + ((chunk ^ (r & 7)) << 4);
+      const long long k = sm.k_at[n & 1][r], v = sm.v_at[n & 1][r];
+      copy16(at, reinterpret_cast<const T*>(p.k) + (k < 0 ? 0 : k) + chunk * 8, k >= 0);
+      copy16(at + kTile * D * 2, reinterpret_cast<const T*>(p.v) + (v < 0 ? 0 : v) + chunk * 8, v >= 0);
+    }
+  };
+
+  // Two tiles' offsets are held: those of the tile that is copied next, and of the one behind it.
+  long long k_next = 0, v_next = 0;
+  for (int n = 0; n < kStages; ++n) {
+    if (n < count) {
+      if (tid < kTile) look_up(sm.k_at[n & 1][tid], sm.v_at[n & 1][tid]);
+      ahead.next(p);
+    }
+    if (n + 1 == kStages) break;  // copied in the first iteration
+    __syncthreads();
+    if (n < count) copy_tile(n);
+    copies_commit();
+    __syncthreads();
+  }
+
+  uint32_t qf[NT][D / 16][2];  // Q^T fragments
+  float o[NT][D / 16][4];      // O^T: dimensions x query rows
+  float top[NT][2], sum[NT][2];
+  int seen[NT][2];             // visible keys of the thread's query rows
+  const float scale2 = p.scale * 1.4426950408889634f;
+  bool fresh = true;
+  for (int n = 0; n < count; ++n) {
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int row = t * 8 + (lane >> 2);
+        const bool in = row < cur.r.lq * group;
+        const T* q = reinterpret_cast<const T*>(p.q) + (in ? (cur.r.q0 + row / group) * p.q_tok +
+                                                             (cur.head * group + row % group) * p.q_head : 0);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t* at = reinterpret_cast<const uint32_t*>(q + k * 16 + (lane & 3) * 2);
+          qf[t][k][0] = in ? __ldg(at) : 0u;
+          qf[t][k][1] = in ? __ldg(at + 4) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = t * 8 + (lane & 3) * 2 + i;
+          seen[t][i] = r < cur.r.lq * group ? visible_keys(p, cur.r, r / group) : 0;
+          top[t][i] = kLowest;
+          sum[t][i] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][k][i] = 0.f;
+      }
+    }
+    copies_wait<kStages - 2>();
+    __syncthreads();  // tile n is here, and every warp is done with the stage of tile n - 1
+    if (n + kStages - 1 < count) copy_tile(n + kStages - 1);
+    copies_commit();
+    const bool more = n + kStages < count;
+    if (more && tid < kTile) look_up(k_next, v_next);
+
+    // ---- S^T of the warp's 16 keys ----
+    const uint32_t ks = smem_of(sm.stage[n % kStages]) + warp * 16 * D * 2, vs = ks + kTile * D * 2;
+    float s[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+    {
+      const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t a[4];
+        load_matrix(a, ks + r * (D * 2) + (((k * 2 + (lane >> 4)) ^ (r & 7)) << 4));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) Half<T>::mma(s[t], a, qf[t][k][0], qf[t][k][1]);
+      }
+    }
+    // ---- softmax of the columns (query rows) over the warp's keys ----
+    const int key = cur.tile * kTile + warp * 16 + (lane >> 2);
+    uint32_t pf[NT][2];
+    bool grow = false;
+    float mx[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key + (i >> 1) * 8 >= seen[t][i & 1]) s[t][i] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = fmaxf(s[t][i], s[t][i + 2]);
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        mx[t][i] = x * scale2;
+        grow |= mx[t][i] > top[t][i] + 8.f;
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float m = fmaxf(top[t][i], mx[t][i]);
+          f[i] = exp2_mufu(top[t][i] - m);
+          top[t][i] = m;
+          sum[t][i] *= f[i];
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][k][i] *= f[i & 1];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = exp2_mufu(fmaf(s[t][i], scale2, -top[t][i & 1]));
+        sum[t][i & 1] += e[i];
+      }
+      // S^T has keys in rows; as the second product's B operand P^T wants them along k.
+      pf[t][0] = transpose8x8(Half<T>::pack(e[0], e[1]));
+      pf[t][1] = transpose8x8(Half<T>::pack(e[2], e[3]));
+    }
+    // ---- O^T += V^T P^T ----
+    {
+      const int r = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t a[4];
+        load_matrix_t(a, vs + r * (D * 2) + (((k * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) Half<T>::mma(o[t][k], a, pf[t][0], pf[t][1]);
+      }
+    }
+    if (more) {
+      if (tid < kTile) {
+        sm.k_at[(n + kStages) & 1][tid] = k_next;
+        sm.v_at[(n + kStages) & 1][tid] = v_next;
+      }
+      ahead.next(p);
+    }
+
+    // ---- the pair ends, or the run does ----
+    if (cur.tile + 1 == cur.tiles || n + 1 == count) {
+      const long long first_tile = begin + n - cur.tile;  // of the pair, in the list
+      const long long first = ((first_tile + 1) * ctas - 1) / total;
+      const long long last = ((first_tile + cur.tiles) * ctas - 1) / total;
+      const int parts = (int)(last - first + 1);
+      const int rows = cur.r.lq * group;
+      float* slots = reinterpret_cast<float*>(p.work) + kTokenCounters;
+      const uint64_t slot_floats = token_slot_floats(kRows, D);
+      // The tile's stage is free until the next iteration's copies.
+      float(*joined)[8][D + 4] = reinterpret_cast<float(*)[8][D + 4]>(sm.stage[n % kStages]);
+      static_assert(sizeof(float) * 4 * 8 * (D + 4) <= stage_bytes<D>(), "joined results fit a stage");
+      __syncthreads();
+      float* mine_at = slots + (blockIdx.x == first ? 2 * first + 1 : 2 * (long long)blockIdx.x) * slot_floats;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (t * 8 >= rows) break;
+        // The four warps' results of eight query rows, joined through shared memory.
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = sum[t][i];
+          x += __shfl_xor_sync(0xffffffffu, x, 4);
+          x += __shfl_xor_sync(0xffffffffu, x, 8);
+          x += __shfl_xor_sync(0xffffffffu, x, 16);
+          const int r = (lane & 3) * 2 + i;
+          if (lane < 4) {
+            sm.top[warp][r] = top[t][i];
+            sm.sum[warp][r] = x;
+          }
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            joined[warp][r][k * 16 + (lane >> 2)] = o[t][k][i];
+            joined[warp][r][k * 16 + 8 + (lane >> 2)] = o[t][k][i + 2];
+          }
+        }
+        __syncthreads();
+        const int limit = min(8, rows - t * 8);
+        for (int x = tid; x < limit * D; x += kThreads) {
+          const int r = x / D, d = x % D;
+          const float m = fmaxf(fmaxf(sm.top[0][r], sm.top[1][r]), fmaxf(sm.top[2][r], sm.top[3][r]));
+          float acc = 0.f, l = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float f = exp2_mufu(sm.top[w][r] - m);
+            acc = fmaf(f, joined[w][r][d], acc);
+            l = fmaf(f, sm.sum[w][r], l);
+          }
+          const int row = t * 8 + r;
+          if (parts == 1) {
+            T* out = reinterpret_cast<T*>(p.o) + (cur.r.q0 + row / group) * p.o_tok +
+                     (cur.head * group + row % group) * p.o_head;
+            out[d] = Half<T>::round(l == 0.f ? 0.f : acc / l);
+          } else {
+            float* at = mine_at + row * (D + 2);
+            __stcg(at + d, acc);
+            if (d == 0) {
+              __stcg(at + D, m);
+              __stcg(at + D + 1, l);
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (parts > 1) {
+        int* counter = reinterpret_cast<int*>(p.work) + first;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) sm.last = atomicAdd(counter, 1) == parts - 1;
+        __syncthreads();
+        if (sm.last) {
+          __threadfence();
+          for (int x = tid; x < rows * D; x += kThreads) {
+            const int row = x / D, d = x % D;
+            float m = kLowest, acc = 0.f, l = 0.f;
+            for (int i = 0; i < parts; ++i) {
+              const float* at = slots + (i == 0 ? 2 * first + 1 : 2 * (first + i)) * slot_floats + row * (D + 2);
+              const float pm = __ldcg(at + D), pl = __ldcg(at + D + 1), po = __ldcg(at + d);
+              const float big = fmaxf(m, pm);
+              const float f = exp2_mufu(m - big), g = exp2_mufu(pm - big);
+              acc = acc * f + po * g;
+              l = l * f + pl * g;
+              m = big;
+            }
+            T* out = reinterpret_cast<T*>(p.o) + (cur.r.q0 + row / group) * p.o_tok +
+                     (cur.head * group + row % group) * p.o_head;
+            out[d] = Half<T>::round(l == 0.f ? 0.f : acc / l);
+          }
+          if (tid == 0) *counter = 0;  // as the next launch finds it
+        }
+      }
+      fresh = true;
+    }
+    cur.next(p);
+  }
+}
+
+}  // namespace
+
+#define TB_TOKEN_ENTRY(name, T, D, NT)                                                                       \
+  extern "C" __global__ void __launch_bounds__(kThreads, 2) name(const __grid_constant__ tb::AttnParams p) { \
+    static_assert(sizeof(Shared<D>) + 128 <= tb::token_smem_bytes(D), "shared memory reservation");          \
+    attention_tokens<T, D, NT>(p);                                                                           \
+  }
+
+TB_TOKEN_ENTRY(attention_tokens_bf16_d128_r8, __nv_bfloat16, 128, 1)
+TB_TOKEN_ENTRY(attention_tokens_bf16_d128_r16, __nv_bfloat16, 128, 2)
+TB_TOKEN_ENTRY(attention_tokens_bf16_d128_r32, __nv_bfloat16, 128, 4)
+TB_TOKEN_ENTRY(attention_tokens_f16_d128_r8, __half, 128, 1)
+TB_TOKEN_ENTRY(attention_tokens_f16_d128_r16, __half, 128, 2)
+TB_TOKEN_ENTRY(attention_tokens_f16_d128_r32, __half, 128, 4)
+TB_TOKEN_ENTRY(attention_tokens_bf16_d64_r8, __nv_bfloat16, 64, 1)
+TB_TOKEN_ENTRY(attention_tokens_bf16_d64_r16, __nv_bfloat16, 64, 2)
+TB_TOKEN_ENTRY(attention_tokens_bf16_d64_r32, __nv_bfloat16, 64, 4)
+TB_TOKEN_ENTRY(attention_tokens_f16_d64_r8, __half, 64, 1)
+TB_TOKEN_ENTRY(attention_tokens_f16_d64_r16, __half, 64, 2)
+TB_TOKEN_ENTRY(attention_tokens_f16_d64_r32, __half, 64, 4)
