@@ -101,6 +101,95 @@ bool rows_aligned(const AttnParams& p) {
   return (p.dim == 64 || p.dim == 128) && (kv & 15) == 0 && (q & 3) == 0;
 }
 
+// Whether the tile kernel takes the call: 16-byte rows of Q and the output too, a group that
+// fits a tile, and pages that cut a 128-key tile evenly (or are cut by it).
+bool tiles_fit(const AttnParams& p) {
+  const uint64_t qo = p.q | p.o | (uint64_t)(2 * (p.q_tok | p.q_head | p.o_tok | p.o_head));
+  const bool pages = !p.table || (p.page >= 8 && 128 % p.page == 0) || p.page % 128 == 0;
+  return rows_aligned(p) && (qo & 15) == 0 && p.heads / p.kv_heads <= 128 && pages;
+}
+
+// A map of rows of `dim` elements with up to three outer dimensions, copied in boxes of 64
+// elements x `box`, 128-byte swizzled. A dimension of extent one may have a step of 0 here;
+// the map wants some multiple of 16 bytes.
+tb_status tmap_rows(CUtensorMap* map, uint32_t dtype, uint64_t base, int rank, const uint64_t* extents,
+                    const int64_t* steps, const uint32_t* box) {
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t boxes[4] = {64, 1, 1, 1}, elem[4] = {1, 1, 1, 1};
+  dims[0] = extents[0];
+  for (int i = 1; i < rank; ++i) {
+    dims[i] = extents[i];
+    strides[i - 1] = steps[i] ? (cuuint64_t)steps[i] * 2 : extents[0] * 2;
+    boxes[i] = box[i];
+    if (strides[i - 1] >= (1ull << 40)) return unsupported("attention strides of 2^40 bytes and more are not implemented");
+  }
+  TB_CU("cuTensorMapEncodeTiled",
+        driver()->cuTensorMapEncodeTiled(
+            map, dtype == TB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+            reinterpret_cast<void*>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
+  return TB_OK;
+}
+
+// Tensor-core kernel for all requests but the token kernel's. `longest`: query rows of a request
+// at most.
+tb_status launch_tiles(Session* s, Stream* st, AttnCall* c, uint64_t longest) {
+  AttnParams& p = c->p;
+  const std::string suffix = std::string(c->dtype == TB_BF16 ? "bf16" : "f16") + "_d" + std::to_string(p.dim);
+  const std::string entry = "attention_tiles_" + suffix;
+  CUfunction fn = nullptr;
+  tb_status rc = builtin_function(s, "attn_tiles", entry.c_str(), &fn);
+  if (rc) return rc;
+  // The kernel's warpgroups re-divide the registers the CTA was launched with; a launch
+  // with fewer than it assumes would leave the softmax warpgroups waiting for registers.
+  int regs = 0;
+  TB_CU("cuFuncGetAttribute", driver()->cuFuncGetAttribute(&regs, CU_FUNC_ATTRIBUTE_NUM_REGS, fn));
+  if (regs < kTileLaunchRegs)
+    return unsupported(entry + " was built with fewer registers than its warpgroups share");
+  const int group = p.heads / p.kv_heads;
+  p.tile_tokens = 128 / group;
+  CUtensorMap mq, mk, mv;
+  const uint64_t q_ext[] = {(uint64_t)p.dim, (uint64_t)p.heads, (uint64_t)p.tq};
+  const int64_t q_steps[] = {1, p.q_head, p.q_tok};
+  const uint32_t q_box[] = {64, (uint32_t)group, (uint32_t)p.tile_tokens};
+  const uint64_t kv_ext[] = {(uint64_t)p.dim, (uint64_t)p.kv_heads, (uint64_t)(p.table ? p.page : p.tk),
+                             (uint64_t)(p.table ? p.pages : 1)};
+  const int64_t k_steps[] = {1, p.k_head, p.k_tok, p.k_page}, v_steps[] = {1, p.v_head, p.v_tok, p.v_page};
+  const uint32_t kv_box[] = {64, 1, (uint32_t)(p.table ? std::min(p.page, 128) : 128), 1};
+  if ((rc = tmap_rows(&mq, c->dtype, p.q, 3, q_ext, q_steps, q_box)) ||
+      (rc = tmap_rows(&mk, c->dtype, p.k, 4, kv_ext, k_steps, kv_box)) ||
+      (rc = tmap_rows(&mv, c->dtype, p.v, 4, kv_ext, v_steps, kv_box)))
+    return rc;
+  // Items (pairs of tiles x key heads) at most: every request may end inside a pair.
+  const uint64_t rows = 2ull * p.tile_tokens, tq = (uint64_t)p.tq, batch = (uint64_t)p.batch;
+  const uint64_t pairs = std::min(tq / rows + std::min(batch, tq), batch * ((longest + rows - 1) / rows));
+  uint64_t grid = pairs * (uint64_t)p.kv_heads;
+  if (grid > 0x7fffffffull) return contract("attention grid exceeds 2^31 CTAs");
+  // Keys are cut into parts where the items cannot fill half of the SMs and there are keys
+  // enough for two parts of two tiles.
+  const uint64_t keys = p.table ? (uint64_t)p.width * p.page : (uint64_t)p.tk;
+  p.splits = (int32_t)std::min<uint64_t>(kTileMaxSplits, keys / 256);
+  p.work = 0;
+  if (p.splits > 1 && grid * 2 <= (uint64_t)s->sm_count) {
+    grid = (uint64_t)s->sm_count;
+    CUdeviceptr work = 0;
+    if ((rc = stream_workspace(s, st, tile_workspace_bytes((int)grid, p.dim), &work))) return rc;
+    p.work = work;
+  }
+  CUdeviceptr status = s->status.device;
+  void* params[] = {&p, &mq, &mk, &mv, &status};
+  rc = launch_builtin(s, st, fn, (unsigned)grid, 1, 1, kTileThreads, (unsigned)tile_smem_bytes(p.dim), params,
+                      entry.c_str());
+  if (rc || !p.work) return rc;
+  const std::string join = "attention_tiles_join_" + suffix;
+  if ((rc = builtin_function(s, "attn_tiles", join.c_str(), &fn))) return rc;
+  int slots = (int)grid;
+  void* join_params[] = {&p, &slots};
+  if ((rc = launch_builtin(s, st, fn, (unsigned)s->sm_count, 1, 1, 256, 0, join_params, join.c_str()))) return rc;
+  note_candidate(entry.c_str());
+  return TB_OK;
+}
+
 // Decode kernel for the requests of at most p.token_rows (row, head) pairs per key head.
 tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
   const std::string entry = std::string("attention_tokens_") + (c->dtype == TB_BF16 ? "bf16" : "f16") + "_d" +
@@ -122,8 +211,13 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
   if (rc) return rc;
   c->p.causal = a.causal ? 1 : 0;
   c->p.scale = (float)(a.scale > 0.0 ? a.scale : 1.0 / std::sqrt((double)c->p.dim));
-  if (a.candidate && strcmp(a.candidate, "attention_rows") != 0)
+  const bool only_rows = a.candidate && strcmp(a.candidate, "attention_rows") == 0;
+  const bool only_tiles = a.candidate && strcmp(a.candidate, "attention_tiles") == 0;
+  if (a.candidate && !only_rows && !only_tiles)
     return contract(std::string("unknown ") + op + " candidate " + a.candidate);
+  const bool tiles = !only_rows && tiles_fit(c->p);
+  if (only_tiles && !tiles)
+    return unsupported("candidate attention_tiles does not take this shape, page size or alignment");
   std::lock_guard<std::mutex> lock(st->enqueue);
   const uint64_t group = (uint64_t)(c->p.heads / c->p.kv_heads);
   const uint64_t longest = a.max_query && a.max_query < (uint64_t)c->p.tq ? a.max_query : (uint64_t)c->p.tq;
@@ -133,7 +227,7 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
     c->p.token_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     if ((rc = launch_tokens(s, st, c)) || longest * group <= (uint64_t)c->p.token_rows) return rc;
   }
-  return launch_rows(s, st, c);
+  return tiles ? launch_tiles(s, st, c, longest) : launch_rows(s, st, c);
 }
 
 }  // namespace

@@ -34,7 +34,9 @@ struct AttnParams {
   int32_t token_rows;      // requests of at most this many (query row, head) pairs per key head
                            // belong to the token kernel, the others to the kernel beside it
   float scale;             // factor of q . k
-  uint64_t work;           // the token kernel's workspace: counters, then partial results
+  uint64_t work;           // workspace: the token kernel's, or the tile kernel's (0: no splitting)
+  int32_t tile_tokens;     // query rows of a 128-row tile, 128 / (heads / kv_heads)
+  int32_t splits;          // the tile kernel cuts a pair's keys into at most this many parts
 };
 
 // Layout of the token kernel's workspace: a counter per CTA, at the same place for every form
@@ -52,6 +54,27 @@ TB_BOTH constexpr uint64_t token_workspace_bytes(int ctas, int rows, int dim) {
 constexpr int kTokenTile = 64, kTokenStages = 3, kTokenThreads = 128;
 TB_BOTH constexpr int token_smem_bytes(int dim) {
   return kTokenStages * 2 * kTokenTile * dim * 2 + 2 * kTokenTile * 16 + 2 * 4 * 8 * 4 + 128 + 128;
+}
+
+// The tile kernel's workspace, behind the token kernel's counters: what the joining kernel
+// reads (the parts of an item, per row; where the row goes), then the partial results.
+//   head:   int32 {items, parts per item}
+//   places: int64 element offset of each row in the output, -1 for no row (items x 256)
+//   stats:  float2 {maximum, sum} (items x parts x 256)
+//   rows:   float [dim] (items x parts x 256)
+// `slots` (items x parts) is at most the SM count.
+constexpr int kTileRows = 256;  // two tiles of 128 (query row, head) pairs
+TB_BOTH constexpr uint64_t tile_places_at() { return 4ull * kTokenCounters + 256; }
+TB_BOTH constexpr uint64_t tile_stats_at(int slots) { return tile_places_at() + 8ull * kTileRows * slots; }
+TB_BOTH constexpr uint64_t tile_rows_at(int slots) { return tile_stats_at(slots) + 8ull * kTileRows * slots; }
+TB_BOTH constexpr uint64_t tile_workspace_bytes(int slots, int dim) {
+  return tile_rows_at(slots) + 4ull * kTileRows * slots * dim;
+}
+constexpr int kTileMaxSplits = 32;
+constexpr int kTileThreads = 384, kTileLaunchRegs = 168;
+constexpr int kTileBarrierBytes = 256, kTileScratchBytes = 256;
+TB_BOTH constexpr int tile_smem_bytes(int dim) {
+  return 6 * 128 * dim * 2 + kTileBarrierBytes + kTileScratchBytes + 1024;
 }
 
 // The index arithmetic is shared by the kernels and a host test of it.
@@ -104,5 +127,61 @@ TB_INDEX_FN int page_of(const AttnParams& p, int b, int index) {
   const int id = load_index(reinterpret_cast<const int*>(p.table) + b * p.table_row + index);
   return id >= 0 && id < p.pages ? id : -1;
 }
+
+#ifdef __CUDACC__
+
+// A thread's stretch of the requests, and the units (tiles of work) before and in it: every
+// thread of the block adds up units(b) over its stretch and a scan joins the sums. `scan`
+// holds one word a warp. Ends with a barrier.
+struct Stretch {
+  int lo, hi;
+  long long before, total;
+};
+
+template <int kThreads, typename Units>
+__device__ __forceinline__ Stretch count_units(int batch, long long* scan, Units units) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Stretch s;
+  const int per = (batch + kThreads - 1) / kThreads;
+  s.lo = min((int)threadIdx.x * per, batch);
+  s.hi = min(s.lo + per, batch);
+  long long mine = 0;
+  for (int b = s.lo; b < s.hi; ++b) mine += units(b);
+  long long upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += x;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  s.before = upto - mine;
+  s.total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) s.before += scan[w];
+    s.total += scan[w];
+  }
+  return s;
+}
+
+// The thread whose stretch holds unit `target` writes its request and the units before that
+// request. Ends with a barrier; `target` lies below the total.
+template <typename Units>
+__device__ __forceinline__ void find_unit(const Stretch& s, long long target, Units units, int* found,
+                                          long long* found_before) {
+  long long at = s.before;
+  for (int b = s.lo; b < s.hi && at <= target; ++b) {
+    const long long n = units(b);
+    if (target < at + n) {
+      *found = b;
+      *found_before = at;
+    }
+    at += n;
+  }
+  __syncthreads();
+}
+
+#endif
 
 }  // namespace tb

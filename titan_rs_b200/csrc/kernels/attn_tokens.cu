@@ -138,42 +138,15 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = p.heads / p.kv_heads;
 
-  // ---- this CTA's run of tiles: every thread adds up a stretch of requests ----
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  const int lo = min(tid * per, p.batch), hi = min(lo + per, p.batch);
-  long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += tiles_of(p, request_of(p, b));
-  long long upto = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += x;
-  }
-  if (lane == 31) sm.scan[warp] = upto;
-  __syncthreads();
-  long long before = upto - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += sm.scan[w];
-    total += sm.scan[w];
-  }
-  total *= p.kv_heads;
+  // ---- this CTA's run of tiles ----
+  const auto units = [&](int b) { return tiles_of(p, request_of(p, b)); };
+  const Stretch stretch = count_units<kThreads>(p.batch, sm.scan, units);
+  const long long total = stretch.total * p.kv_heads;
   const long long ctas = min((long long)gridDim.x, total);
   if (blockIdx.x >= ctas) return;
   const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
-  {
-    // The request that holds tile `begin`: its requests' tiles start at kv_heads x (tiles before).
-    long long at = before;
-    for (int b = lo; b < hi; ++b) {
-      const int n = tiles_of(p, request_of(p, b));
-      if (at * p.kv_heads <= begin && begin < (at + n) * p.kv_heads) {
-        sm.found_b = b;
-        sm.found_before = at;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
+  // The tiles of a request start at kv_heads x (tiles before it).
+  find_unit(stretch, begin / p.kv_heads, units, &sm.found_b, &sm.found_before);
   Cursor cur;
   cur.seek(p, sm.found_b);
   {
