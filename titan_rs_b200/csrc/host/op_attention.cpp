@@ -164,23 +164,23 @@ tb_status launch_tiles(Session* s, Stream* st, AttnCall* c, uint64_t longest) {
   const uint64_t rows = 2ull * p.tile_tokens, tq = (uint64_t)p.tq, batch = (uint64_t)p.batch;
   const uint64_t pairs = std::min(tq / rows + std::min(batch, tq), batch * ((longest + rows - 1) / rows));
   uint64_t grid = pairs * (uint64_t)p.kv_heads;
-  if (grid > 0x7fffffffull) return contract("attention grid exceeds 2^31 CTAs");
+  if (grid > 0x3fffffffull) return contract("attention work list exceeds 2^30 items");
+  p.max_items = (int32_t)grid;
   // Keys are cut into parts where the items cannot fill half of the SMs and there are keys
   // enough for two parts of two tiles.
   const uint64_t keys = p.table ? (uint64_t)p.width * p.page : (uint64_t)p.tk;
-  p.splits = (int32_t)std::min<uint64_t>(kTileMaxSplits, keys / 256);
-  p.work = 0;
-  if (p.splits > 1 && grid * 2 <= (uint64_t)s->sm_count) {
-    grid = (uint64_t)s->sm_count;
-    CUdeviceptr work = 0;
-    if ((rc = stream_workspace(s, st, tile_workspace_bytes((int)grid, p.dim), &work))) return rc;
-    p.work = work;
-  }
+  const uint64_t sms = (uint64_t)s->sm_count;
+  p.splits = grid * 2 <= sms ? (int32_t)std::min<uint64_t>(kTileMaxSplits, keys / 256) : 1;
+  grid = p.splits > 1 ? sms : std::min(grid, sms);  // one CTA an SM, drawing items until there are no more
+  CUdeviceptr work = 0;
+  const size_t bytes = p.splits > 1 ? tile_workspace_bytes((int)grid, p.dim) : 4ull * kTokenCounters;
+  if ((rc = stream_workspace(s, st, bytes, &work))) return rc;
+  p.work = work;
   CUdeviceptr status = s->status.device;
   void* params[] = {&p, &mq, &mk, &mv, &status};
   rc = launch_builtin(s, st, fn, (unsigned)grid, 1, 1, kTileThreads, (unsigned)tile_smem_bytes(p.dim), params,
                       entry.c_str());
-  if (rc || !p.work) return rc;
+  if (rc || p.splits <= 1) return rc;
   const std::string join = "attention_tiles_join_" + suffix;
   if ((rc = builtin_function(s, "attn_tiles", join.c_str(), &fn))) return rc;
   int slots = (int)grid;
@@ -197,7 +197,7 @@ tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
   CUfunction fn = nullptr;
   tb_status rc = builtin_function(s, "attn_tokens", entry.c_str(), &fn);
   if (rc) return rc;
-  const int ctas = std::min(2 * s->sm_count, kTokenCounters);  // two resident on each SM
+  const int ctas = std::min(2 * s->sm_count, kTileNext);  // two resident on each SM
   CUdeviceptr work = 0;
   if ((rc = stream_workspace(s, st, token_workspace_bytes(ctas, c->p.token_rows, c->p.dim), &work))) return rc;
   c->p.work = work;

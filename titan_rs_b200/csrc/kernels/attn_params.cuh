@@ -34,16 +34,18 @@ struct AttnParams {
   int32_t token_rows;      // requests of at most this many (query row, head) pairs per key head
                            // belong to the token kernel, the others to the kernel beside it
   float scale;             // factor of q . k
-  uint64_t work;           // workspace: the token kernel's, or the tile kernel's (0: no splitting)
+  uint64_t work;           // workspace of the token and tile kernels
   int32_t tile_tokens;     // query rows of a 128-row tile, 128 / (heads / kv_heads)
-  int32_t splits;          // the tile kernel cuts a pair's keys into at most this many parts
+  int32_t max_items;       // (pair of tiles, key head) items of sound index tensors at most
+  int32_t splits;          // the tile kernel cuts a pair's keys into at most this many parts; with
+                           // more than one, the workspace has room for gridDim.x of them
 };
 
 // Layout of the token kernel's workspace: a counter per CTA, at the same place for every form
 // of the kernel (it is zero between launches), then two partial results a CTA (its first
 // request may have begun in an earlier CTA, its last may go on in a later one), each
 // rows x (dim + 2) floats: O, then the row's maximum and sum.
-constexpr int kTokenCounters = 1024;  // CTAs at most
+constexpr int kTokenCounters = 1024;  // the token kernel's CTAs, and two of the tile kernel
 TB_BOTH constexpr uint64_t token_slot_floats(int rows, int dim) { return (uint64_t)rows * (dim + 2); }
 TB_BOTH constexpr uint64_t token_workspace_bytes(int ctas, int rows, int dim) {
   return 4ull * kTokenCounters + 2ull * ctas * token_slot_floats(rows, dim) * 4;
@@ -72,10 +74,14 @@ TB_BOTH constexpr uint64_t tile_workspace_bytes(int slots, int dim) {
 }
 constexpr int kTileMaxSplits = 32;
 constexpr int kTileThreads = 384, kTileLaunchRegs = 168;
-constexpr int kTileBarrierBytes = 256, kTileScratchBytes = 256;
+constexpr int kTileBarrierBytes = 256, kTileScratchBytes = 512;
+// Three Q tiles, two stages of a K and a V tile, barriers and item descriptions.
 TB_BOTH constexpr int tile_smem_bytes(int dim) {
-  return 6 * 128 * dim * 2 + kTileBarrierBytes + kTileScratchBytes + 1024;
+  return 7 * 128 * dim * 2 + kTileBarrierBytes + kTileScratchBytes + 1024;
 }
+// The tile kernel's work counter and its count of finished CTAs, the last two of the counters
+// at the workspace's front.
+constexpr int kTileNext = kTokenCounters - 2, kTileDone = kTokenCounters - 1;
 
 // The index arithmetic is shared by the kernels and a host test of it.
 #ifdef __CUDACC__

@@ -43,27 +43,45 @@ constexpr uint32_t kFailProducer = 0x56010000u;
 constexpr uint32_t kFailMma = 0x56020000u;
 constexpr uint32_t kFailSoftmax = 0x56030000u;
 constexpr uint32_t kFailClear = 0x56040000u;
-constexpr uint32_t kControlRegs = 56, kSoftmaxRegs = 216;
+constexpr uint32_t kFailSchedule = 0x56050000u;
+constexpr uint32_t kControlRegs = 72, kSoftmaxRegs = 216;
 static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kTileThreads * kTileLaunchRegs,
               "the warpgroups' registers exceed the launch allocation");
 
+constexpr int kSlots = 4;         // item descriptions in flight
+constexpr int kItemReaders = 11;  // warps 0, 1, 2 and the eight softmax warps
+constexpr int kQ = 3;             // Q tiles in shared memory
+
 struct Barriers {
-  uint64_t q_full;
-  uint64_t kv_full[2], kv_empty[2];  // stage j & 1 holds K_j and V_{j-1}
+  uint64_t q_full[kQ], q_empty[kQ];
+  uint64_t kv_full[2], kv_empty[2];  // the stage of step t holds K of its key tile and V of the one before
   uint64_t s_full[2];                // per query tile (A, B)
   uint64_t p_half[2];                // per query tile: P of keys [0, 64) is in TMEM
   uint64_t p_full[2];                // per query tile: P of keys [64, 128) is in TMEM
-  uint64_t v_raw;                    // the last V tile, before its rows past the end are cleared
-  uint64_t o_final;
+  uint64_t o_full[2];                // per query tile: an item's last product is done
+  uint64_t v_raw[2];                 // per stage: a V tile whose rows past the end warp 2 clears
   uint64_t drain;
+  uint64_t item_full[kSlots], item_empty[kSlots];
+  uint64_t item_want;                // the producer nears its item's end: draw the next one
   uint32_t tmem_base;
 };
 static_assert(sizeof(Barriers) <= kTileBarrierBytes, "barrier block overflows its reservation");
 
+// One item: two query tiles of one request and key head, and a range of key tiles.
+struct Item {
+  int n, n_a, n_b;       // key tiles of the part, and how many of them tiles A and B need; n < 0: no more items
+  int lo;                // the first key tile
+  int hk, b;             // key head, request
+  int row, valid;        // tile A's first row of q, and rows from there to the request's end
+  int base;              // local row i sees base + i keys (causal)
+  int lk, k0;            // keys of the request, and its first row of k (packed)
+  int last_rows;         // rows of the last key tile if it runs past the request's end, else 0
+  int index, part;       // item number and part
+};
+
 struct Scratch {
+  Item items[kSlots];
   long long scan[kTileThreads / 32];
-  long long found_before;
-  int found;
 };
 static_assert(sizeof(Scratch) <= kTileScratchBytes, "scratch block overflows its reservation");
 
@@ -176,12 +194,40 @@ __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, i
   if (lane == 0) mbar_arrive(p_full);
 }
 
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+// A warp's place in the list of items: it reads each description and lets go of its slot.
+struct Reader {
+  int slot = 0;
+  uint32_t phase = 0;
+
+  // Called by all lanes of the warp, or (kLanes = 1) by one; false when the wait ran out.
+  template <int kLanes = 32>
+  __device__ __forceinline__ bool next(Barriers* bars, const Scratch* scratch, Item& item) {
+    bool ok = mbar_wait(&bars->item_full[slot], phase);
+    if (kLanes > 1) ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      item = scratch->items[slot];
+      if (kLanes > 1) __syncwarp();
+      if (kLanes == 1 || lane_id() == 0) mbar_arrive(&bars->item_empty[slot]);
+      if (++slot == kSlots) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+    return ok;
+  }
+};
+
 template <typename T, int HD>
 __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUtensorMap& tmap_q,
                                                 const CUtensorMap& tmap_k, const CUtensorMap& tmap_v,
                                                 uint32_t* status) {
   using S = Shape<T, HD>;
-  constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * S::kTileBytes, OFF_V = OFF_K + 2 * S::kTileBytes,
+  constexpr int OFF_Q = 0, OFF_K = OFF_Q + kQ * S::kTileBytes, OFF_V = OFF_K + 2 * S::kTileBytes,
                 OFF_BAR = OFF_V + 2 * S::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -189,55 +235,44 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
   Scratch* scratch = reinterpret_cast<Scratch*>(smem + OFF_BAR + kTileBarrierBytes);
   const int warp = warp_id(), lane = lane_id();
   const int group = p.heads / p.kv_heads;
-
-  // ---- this CTA's item: (pair of tiles, key head, part), the longest rows first ----
-  const auto units = [&](int b) { return pairs_of(p, request_of(p, b)); };
-  const Stretch stretch = count_units<kTileThreads>(p.batch, scratch->scan, units);
-  const long long items = stretch.total * p.kv_heads;
-  // Parts of an item: as many as fill the SMs, when the caller gave a workspace for them.
-  const int parts = p.work && items > 0 ? (int)max(1ll, min((long long)p.splits, gridDim.x / items)) : 1;
-  if (p.work && blockIdx.x == 0 && threadIdx.x == 0) {
-    int* head = reinterpret_cast<int*>(p.work + 4ull * kTokenCounters);
-    head[0] = parts > 1 ? (int)items : 0;
-    head[1] = parts;
-  }
-  const long long item = blockIdx.x / parts;
-  const int part = blockIdx.x % parts;
-  if (item >= items) return;
-  const long long unit = stretch.total - 1 - item / p.kv_heads;
-  const int hk = (int)(item % p.kv_heads);
-  find_unit(stretch, unit, units, &scratch->found, &scratch->found_before);
-  const int b = scratch->found;
-  const AttnRequest r = request_of(p, b);
-  const int tok0 = (int)(unit - scratch->found_before) * 2 * p.tile_tokens;  // tile A's first query row
-  const bool has_b = tok0 + p.tile_tokens < r.lq;
-  // Key tiles that each tile needs (of its last row), and this part's range of them.
-  const int end_a = (visible_keys(p, r, min(tok0 + p.tile_tokens, r.lq) - 1) + BN - 1) / BN;
-  const int end_b = has_b ? (visible_keys(p, r, min(tok0 + 2 * p.tile_tokens, r.lq) - 1) + BN - 1) / BN : 0;
-  const int all = max(end_a, end_b);
-  const int lo = (int)((long long)part * all / parts), hi = (int)((long long)(part + 1) * all / parts);
-  const int n_a = max(0, min(hi, end_a) - lo), n_b = max(0, min(hi, end_b) - lo), n = hi - lo;
-  // Whether this part's last key tile runs past the request's end.
-  const int last_rows = r.lk % BN;
-  const bool clear = last_rows && n > 0 && hi == r.lk / BN + 1;
+  int* const counters = reinterpret_cast<int*>(p.work);
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, 1);
+    for (int i = 0; i < kQ; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_empty[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->kv_full[i], 1);
       mbar_init(&bars->kv_empty[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_half[i], 4);
       mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->o_full[i], 1);
+      mbar_init(&bars->v_raw[i], 1);
     }
-    mbar_init(&bars->v_raw, 1);
-    mbar_init(&bars->o_final, 1);
     mbar_init(&bars->drain, 1);
+    mbar_init(&bars->item_want, 1);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&bars->item_full[i], 1);
+      mbar_init(&bars->item_empty[i], kItemReaders);
+    }
     fence_barrier_init();
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
+  }
+  const auto units = [&](int b) { return pairs_of(p, request_of(p, b)); };
+  const Stretch stretch = count_units<kTileThreads>(p.batch, scratch->scan, units);
+  // (More than max_items only where cu_seqlens counts rows twice; the rest is then left.)
+  const long long items = min(stretch.total * p.kv_heads, (long long)p.max_items);
+  // Parts of an item: as many as fill the SMs, where the workspace has room for them.
+  const int parts = p.splits > 1 && items > 0 ? (int)max(1ll, min((long long)p.splits, gridDim.x / items)) : 1;
+  if (p.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) {
+    int* head = counters + kTokenCounters;
+    head[0] = parts > 1 ? (int)items : 0;
+    head[1] = parts;
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -246,146 +281,334 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
 
   if (warp < 4) {
     setmaxnreg_dec<kControlRegs>();
-    if (warp == 0 && n > 0) {
+    if (warp == 3) {
+      // ---------------- items: the longest rows first, drawn from a counter ----------------
+      long long w = blockIdx.x;
+      int b = p.batch;                   // the walk stands before request b,
+      long long before = stretch.total;  // which has this many units before it
+      for (int k = 0;; ++k) {
+        const int slot = k % kSlots;
+        // An item is drawn only when its predecessor nears its end, so no CTA sits on work that
+        // another could begin.
+        if (!__all_sync(0xffffffffu, (k == 0 || mbar_wait(&bars->item_want, (k - 1) & 1)) &&
+                                         mbar_wait(&bars->item_empty[slot], ((k / kSlots) & 1) ^ 1))) {
+          if (lane == 0) report_status(status, kFailSchedule | 1);
+          break;
+        }
+        if (k > 0) {
+          if (lane == 0) w = (long long)gridDim.x + atomicAdd(counters + kTileNext, 1);
+          w = __shfl_sync(0xffffffffu, w, 0);
+        }
+        const bool more = w < items * parts;
+        Item it{};
+        it.n = -1;
+        if (more) {
+          const long long index = w / parts, unit = stretch.total - 1 - index / p.kv_heads;
+          const int part = (int)(w % parts);
+          // Back over the requests, 32 at a time, to the one that holds `unit`.
+          while (unit < before) {
+            const int mine = b - 1 - lane;
+            const int own = mine >= 0 ? units(mine) : 0;
+            long long upto = own;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+              const long long x = __shfl_up_sync(0xffffffffu, upto, off);
+              if (lane >= off) upto += x;
+            }
+            const uint32_t reached = __ballot_sync(0xffffffffu, before - upto <= unit);
+            const int at = reached ? __ffs(reached) - 1 : 31;
+            before -= __shfl_sync(0xffffffffu, upto, at);
+            b -= at + 1;
+          }
+          const AttnRequest r = request_of(p, b);
+          const int tok0 = (int)(unit - before) * 2 * p.tile_tokens;
+          const bool has_b = tok0 + p.tile_tokens < r.lq;
+          // Key tiles that each tile needs (of its last row), and this part's range of them.
+          const int end_a = (visible_keys(p, r, min(tok0 + p.tile_tokens, r.lq) - 1) + BN - 1) / BN;
+          const int end_b =
+              has_b ? (visible_keys(p, r, min(tok0 + 2 * p.tile_tokens, r.lq) - 1) + BN - 1) / BN : 0;
+          const int all = max(end_a, end_b);
+          const int lo = (int)((long long)part * all / parts), hi = (int)((long long)(part + 1) * all / parts);
+          it.n = hi - lo;
+          it.n_a = max(0, min(hi, end_a) - lo);
+          it.n_b = max(0, min(hi, end_b) - lo);
+          it.lo = lo;
+          it.hk = (int)(index % p.kv_heads);
+          it.b = b;
+          it.row = r.q0 + tok0;
+          it.valid = r.lq - tok0;
+          it.base = p.causal ? r.lk - r.lq + tok0 + 1 : r.lk;
+          it.lk = r.lk;
+          it.k0 = r.k0;
+          it.last_rows = it.n > 0 && hi == r.lk / BN + 1 ? r.lk % BN : 0;
+          it.index = (int)index;
+          it.part = part;
+        }
+        if (lane == 0) {
+          scratch->items[slot] = it;
+          mbar_arrive(&bars->item_full[slot]);
+        }
+        if (!more) break;
+      }
+      // The counters are zero again for the next launch.
+      if (lane == 0 && atomicAdd(counters + kTileDone, 1) == (int)gridDim.x - 1) {
+        counters[kTileNext] = 0;
+        counters[kTileDone] = 0;
+      }
+    } else if (warp == 0) {
       // ---------------- producer ----------------
       if (lane == 0) {
         tma_prefetch_desc(&tmap_q);
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
-        const uint32_t bytes = S::kHalves * p.tile_tokens * group * 128;
-        mbar_arrive_expect_tx(&bars->q_full, bytes * (has_b ? 2 : 1));
-        for (int x = 0; x < (has_b ? 2 : 1); ++x)
-          for (int h = 0; h < S::kHalves; ++h)
-            tma_load_3d(smem + OFF_Q + x * S::kTileBytes + h * S::kHalfBytes, &tmap_q, &bars->q_full, 64 * h,
-                        hk * group, r.q0 + tok0 + x * p.tile_tokens);
       }
-      __syncwarp();
       // Lane i copies box i of a key tile: rows [i box, (i + 1) box) of it.
       const bool paged = p.table != 0;
       const int box = paged ? min(p.page, BN) : BN, boxes = BN / box;
       const bool active = lane < boxes;
-      const int held = paged ? (r.lk + p.page - 1) / p.page : 0;  // pages of the request
       // The coordinates of the lane's box of key tile j: (row, page).
-      const auto row_of = [&](int j) { return paged ? (p.page > BN ? j * BN % p.page : 0) : r.k0 + j * BN; };
-      const auto page_at = [&](int j) {
-        if (!paged || !active || j >= hi) return 0;
+      const auto row_of = [&](const Item& it, int j) {
+        return paged ? (p.page > BN ? j * BN % p.page : 0) : it.k0 + j * BN;
+      };
+      const auto page_at = [&](const Item& it, int j) {
+        if (!paged || !active || j >= it.lo + it.n) return 0;
         const int index = p.page > BN ? (int)((long long)j * BN / p.page) : j * boxes + lane;
-        const int id = index < held ? page_of(p, b, index) : -1;
+        const int id = (long long)index * p.page < it.lk ? page_of(p, it.b, index) : -1;
         return id < 0 ? p.pages : id;
       };
-      const auto load = [&](int off, const CUtensorMap* map, uint64_t* bar, int j, int w) {
+      const auto load = [&](int off, const CUtensorMap* map, uint64_t* bar, int hk, int row, int w) {
         if (!active) return;
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h)
-          tma_load_4d(smem + off + h * S::kHalfBytes + lane * box * 128, map, bar, 64 * h, hk, row_of(j), w);
+          tma_load_4d(smem + off + h * S::kHalfBytes + lane * box * 128, map, bar, 64 * h, hk, row, w);
       };
-      const auto prefetch = [&](int j, int w) {
-        if (!active || j >= hi || (paged && w == p.pages)) return;
+      const auto prefetch = [&](const Item& it, int j, int w) {
+        if (!active || j >= it.lo + it.n || (paged && w == p.pages)) return;
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h) {
-          tma_prefetch_l2_4d(&tmap_k, 64 * h, hk, row_of(j), w);
-          tma_prefetch_l2_4d(&tmap_v, 64 * h, hk, row_of(j), w);
+          tma_prefetch_l2_4d(&tmap_k, 64 * h, it.hk, row_of(it, j), w);
+          tma_prefetch_l2_4d(&tmap_v, 64 * h, it.hk, row_of(it, j), w);
         }
       };
-      int w_old = 0, w_now = page_at(lo), w_next = page_at(lo + 1);
-      uint32_t issued[2] = {0, 0};
-      bool ok = true;
-      for (int it = 0; it <= n; ++it) {
-        const int w_after = page_at(lo + it + 2);
-        prefetch(lo + it + 1, w_next);
-        const int st = it & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->kv_empty[st], ((it >> 1) & 1) ^ 1));
-        if (!ok) {
-          if (lane == 0) report_status(status, kFailProducer | 1);
-          break;
+      int q_slot = 0;
+      uint32_t q_phase = 1;  // of q_empty: the first round finds the slots free
+      uint32_t q_issued[kQ] = {0, 0, 0}, kv_issued[2] = {0, 0};
+      // Query tile x of the item into the next Q slot.
+      const auto load_q = [&](const Item& it, int x) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->q_empty[q_slot], q_phase))) return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->q_full[q_slot], S::kHalves * p.tile_tokens * group * 128);
+          for (int h = 0; h < S::kHalves; ++h)
+            tma_load_3d(smem + OFF_Q + q_slot * S::kTileBytes + h * S::kHalfBytes, &tmap_q, &bars->q_full[q_slot],
+                        64 * h, it.hk * group, it.row + x * p.tile_tokens);
         }
-        const bool has_k = it < n, has_v = it >= 1;
-        // The last iteration brings a V tile only; one to be cleared goes to warp 2 first,
-        // which arrives on kv_full for it.
-        uint64_t* full = clear && it == n ? &bars->v_raw : &bars->kv_full[st];
-        if (lane == 0) mbar_arrive_expect_tx(full, (has_k ? S::kTileBytes : 0) + (has_v ? S::kTileBytes : 0));
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) q_issued[i] += i == q_slot;
+        if (++q_slot == kQ) {
+          q_slot = 0;
+          q_phase ^= 1;
+        }
+        return true;
+      };
+      Reader reader;
+      Item cur{}, nxt{};
+      int j = 0, w_now = 0, w_next = 0, n_w0 = 0, n_w1 = 0;  // pages of the lane's boxes, two key tiles ahead
+      bool has_v = false;  // a V tile is owed: the one of the last step's key tile
+      int v_hk = 0, v_row = 0, v_page = 0, v_clear = 0;
+      uint32_t step = 0;
+      bool ok = true;
+      while (ok) {
+        const bool has_k = cur.n > 0;
+        if (!has_k && !has_v) {
+          if (cur.n < 0) break;
+          ok = reader.next(bars, scratch, cur);
+          if (ok && cur.n == 0 && lane == 0) mbar_arrive(&bars->item_want);
+          w_now = page_at(cur, cur.lo);
+          w_next = page_at(cur, cur.lo + 1);
+          continue;
+        }
+        int w_after = 0;
+        if (has_k) {
+          if (lane == 0 && j == max(0, cur.n - 3)) mbar_arrive(&bars->item_want);
+          w_after = page_at(cur, cur.lo + j + 2);
+          prefetch(cur, cur.lo + j + 1, w_next);
+          if (j == 0 && cur.n_a > 0) ok = load_q(cur, 0);
+          if (j + 1 == cur.n && ok) {
+            // The item behind it, and its first pages, while this step's stage is still in use.
+            // (One item only: everyone has begun the item before this one, so it is there.)
+            ok = reader.next(bars, scratch, nxt);
+            if (ok && nxt.n == 0 && lane == 0) mbar_arrive(&bars->item_want);
+            n_w0 = page_at(nxt, nxt.lo);
+            n_w1 = page_at(nxt, nxt.lo + 1);
+          }
+        }
+        const int st = step & 1;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars->kv_empty[st], ((step >> 1) & 1) ^ 1));
+        if (!ok) break;
+        // A V tile with rows to clear goes to warp 2 first, which arrives on kv_full for the step.
+        const bool raw = has_v && v_clear;
+        if (lane == 0) {
+          const uint32_t k_bytes = has_k ? S::kTileBytes : 0, v_bytes = has_v ? S::kTileBytes : 0;
+          if (raw) {
+            if (k_bytes) mbar_expect_tx(&bars->kv_full[st], k_bytes);
+            mbar_arrive_expect_tx(&bars->v_raw[st], v_bytes);
+          } else {
+            mbar_arrive_expect_tx(&bars->kv_full[st], k_bytes + v_bytes);
+          }
+        }
         __syncwarp();
-        if (has_k) load(OFF_K + st * S::kTileBytes, &tmap_k, full, lo + it, w_now);
-        if (has_v) load(OFF_V + st * S::kTileBytes, &tmap_v, full, lo + it - 1, w_old);
-        ++issued[st];
-        w_old = w_now;
+        if (has_k) load(OFF_K + st * S::kTileBytes, &tmap_k, &bars->kv_full[st], cur.hk, row_of(cur, cur.lo + j), w_now);
+        if (has_v)
+          load(OFF_V + st * S::kTileBytes, &tmap_v, raw ? &bars->v_raw[st] : &bars->kv_full[st], v_hk, v_row, v_page);
+        ++kv_issued[st];
+        ++step;
+        has_v = has_k;
+        if (!has_k) continue;
+        v_hk = cur.hk;
+        v_row = row_of(cur, cur.lo + j);
+        v_page = w_now;
+        v_clear = j + 1 == cur.n && cur.last_rows;
+        if (j == 0 && cur.n_b > 0) ok = load_q(cur, 1);
         w_now = w_next;
         w_next = w_after;
+        if (++j == cur.n) {
+          cur = nxt;
+          j = 0;
+          w_now = n_w0;
+          w_next = n_w1;
+        }
       }
       if (!ok) {
-        if (!mbar_wait(&bars->q_full, 0)) report_status(status, kFailProducer | 3);
-        for (int s = 0; s < 2; ++s)
-          if (issued[s] && !mbar_wait(&bars->kv_full[s], (issued[s] - 1) & 1))
+        if (lane == 0) report_status(status, kFailProducer | 1);
+        for (int i = 0; i < kQ; ++i)
+          if (q_issued[i] && !mbar_wait(&bars->q_full[i], (q_issued[i] - 1) & 1))
+            report_status(status, kFailProducer | 3);
+        for (int i = 0; i < 2; ++i)
+          if (kv_issued[i] && !mbar_wait(&bars->kv_full[i], (kv_issued[i] - 1) & 1))
             report_status(status, kFailProducer | 4);
       }
     } else if (warp == 1) {
-      if (lane == 0 && n > 0) {
-        // ---------------- MMA issuer ----------------
-        bool ok = mbar_wait(&bars->q_full, 0);
-        if (!ok) report_status(status, kFailMma | 1);
-        const uint64_t qd_a = sdesc_sw128(smem_addr(smem + OFF_Q), 16, 1024);
-        const uint64_t qd_b = sdesc_sw128(smem_addr(smem + OFF_Q + S::kTileBytes), 16, 1024);
+      // ---------------- MMA issuer ----------------
+      // Step t: the products P V of the key tile before, then the scores Q K^T of this one,
+      // per query tile. The step that begins an item ends the one before it, unless that has
+      // no keys (or there is none): then a step without scores comes between.
+      if (lane == 0) {
+        Reader reader;
+        Item it{};
+        bool ok = true, owed = false;
+        int n = 0, n_a = 0, n_b = 0, j = 0;
+        int pj = 0, pn_a = 0, pn_b = 0;  // the key tile before: its number in its item, and the tiles that need it
+        const uint64_t qd0 = sdesc_sw128(smem_addr(smem + OFF_Q), 16, 1024);
         const uint64_t kd0 = sdesc_sw128(smem_addr(smem + OFF_K), 16, 1024);
         const uint64_t vd0 = sdesc_sw128(smem_addr(smem + OFF_V), S::kHalfBytes, 1024);
-        for (int j = 0; j <= n && ok; ++j) {
-          const int st = j & 1;
+        int q_a = 0, q_b = 0, q_slot = 0;
+        uint32_t q_phase = 0, step = 0, s_a = 0, s_b = 0;
+        while (ok) {
+          if (n <= 0 && !owed) {
+            if (n < 0) break;
+            ok = reader.next<1>(bars, scratch, it);
+            n = it.n;
+            n_a = it.n_a;  // 0 in an item without keys, and behind the last one
+            n_b = it.n_b;
+            continue;
+          }
+          const int st = step & 1;
           const uint64_t kd = desc_add(kd0, st * (S::kTileBytes >> 4));
           const uint64_t vd = desc_add(vd0, st * (S::kTileBytes >> 4));
-          if (!mbar_wait(&bars->kv_full[st], (j >> 1) & 1)) {
+          if (!mbar_wait(&bars->kv_full[st], (step >> 1) & 1)) {
             report_status(status, kFailMma | 2);
             ok = false;
             break;
           }
-          for (int x = 0; x < 2; ++x) {
-            const int nx = x ? n_b : n_a;
+          const auto tile = [&](auto which, int nx, int pnx, int& q_at, uint32_t& scores) {
+            constexpr int x = decltype(which)::value;
             const uint32_t s_tmem = tmem + x * BN, o_tmem = tmem + (2 + x) * BN;
-            if (j >= 1 && j - 1 < nx) {
+            if (pj < pnx) {
+              const uint32_t parity = (scores - 1) & 1;
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                if (!mbar_wait(half ? &bars->p_full[x] : &bars->p_half[x], (j - 1) & 1)) {
+                if (!mbar_wait(half ? &bars->p_full[x] : &bars->p_half[x], parity)) {
                   report_status(status, kFailMma | 3);
-                  ok = false;
-                  break;
+                  return false;
                 }
                 tc_fence_after_sync();
 #pragma unroll
                 for (int k = 4 * half; k < 4 * half + 4; ++k)
                   umma_bf16_ts(o_tmem, s_tmem + k * 8, desc_add(vd, k * (2048 >> 4)), S::kIdescO,
-                               (k > 0 || j > 1) ? 1u : 0u);
+                               (k > 0 || pj > 0) ? 1u : 0u);
               }
-              if (!ok) break;
+              if (pj + 1 == pnx) umma_commit(&bars->o_full[x]);
             }
             if (j < nx) {
+              if (j == 0) {
+                if (!mbar_wait(&bars->q_full[q_slot], q_phase)) {
+                  report_status(status, kFailMma | 1);
+                  return false;
+                }
+                q_at = q_slot;
+                if (++q_slot == kQ) {
+                  q_slot = 0;
+                  q_phase ^= 1;
+                }
+              }
+              const uint64_t qd = desc_add(qd0, q_at * (S::kTileBytes >> 4));
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k) {
                 const uint32_t off = (k >> 2) * (S::kHalfBytes >> 4) + (k & 3) * 2;
-                umma_bf16_ss(s_tmem, desc_add(x ? qd_b : qd_a, off), desc_add(kd, off), S::kIdescS, k > 0 ? 1u : 0u);
+                umma_bf16_ss(s_tmem, desc_add(qd, off), desc_add(kd, off), S::kIdescS, k > 0 ? 1u : 0u);
               }
               umma_commit(&bars->s_full[x]);
+              ++scores;
+              if (j + 1 == nx) umma_commit(&bars->q_empty[q_at]);
             }
-          }
+            return true;
+          };
+          ok = tile(Int<0>(), n_a, pn_a, q_a, s_a) && tile(Int<1>(), n_b, pn_b, q_b, s_b);
           if (!ok) break;
           umma_commit(&bars->kv_empty[st]);
+          ++step;
+          owed = n > 0;
+          pj = j;
+          pn_a = n_a;
+          pn_b = n_b;
+          if (owed && ++j == n) {
+            ok = reader.next<1>(bars, scratch, it);
+            n = it.n;
+            n_a = it.n_a;
+            n_b = it.n_b;
+            j = 0;
+          }
         }
-        umma_commit(&bars->o_final);
         umma_commit(&bars->drain);
         if (!mbar_wait(&bars->drain, 0)) report_status(status, kFailMma | 5);
       }
-    } else if (warp == 2 && clear) {
-      // ---------------- rows of the last V tile past the request's end ----------------
-      const int st = n & 1;
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_raw, 0));
-      if (ok) {
-        const int words = (BN - last_rows) * 8;  // 16-byte words of one half
+    } else {
+      // ---------------- rows of an item's last V tile past the request's end ----------------
+      Reader reader;
+      Item it;
+      uint32_t step = 0, cleared[2] = {0, 0};
+      bool owed = false;
+      while (reader.next(bars, scratch, it) && it.n >= 0) {
+        if (it.n == 0 && owed) ++step;  // the step without scores
+        owed = it.n > 0;
+        step += it.n;
+        if (it.last_rows == 0) continue;
+        // Its V tile comes with the step behind the item's last key tile.
+        const int st = step & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_raw[st], (st ? cleared[1] : cleared[0]) & 1))) {
+          if (lane == 0) report_status(status, kFailClear | 1);
+          break;
+        }
+        ++(st ? cleared[1] : cleared[0]);
+        const int words = (BN - it.last_rows) * 8;  // 16-byte words of one half
         for (int h = 0; h < S::kHalves; ++h) {
-          uint4* at = reinterpret_cast<uint4*>(smem + OFF_V + st * S::kTileBytes + h * S::kHalfBytes + last_rows * 128);
+          uint4* at =
+              reinterpret_cast<uint4*>(smem + OFF_V + st * S::kTileBytes + h * S::kHalfBytes + it.last_rows * 128);
           for (int i = lane; i < words; i += 32) at[i] = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->kv_full[st]);
-      } else if (lane == 0) {
-        report_status(status, kFailClear | 1);
       }
     }
   } else {
@@ -397,37 +620,44 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + lane_off + x * BN;
     const uint32_t o_tmem = tmem + lane_off + (2 + x) * BN;
-    const int i = tok0 + x * p.tile_tokens + row / group;  // the query row in its request
-    const bool in = row < p.tile_tokens * group && i < r.lq;
-    // Rows of no query compute on whatever is there and are not stored.
-    const int seen = in ? visible_keys(p, r, i) : r.lk;
-    const int nx = x ? n_b : n_a;
+    const int i = x * p.tile_tokens + row / group;  // the query row, from tile A's first
+    const bool used = row < p.tile_tokens * group;
     const float scale2 = p.scale * 1.4426950408889634f;
-    float m = kLowest, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < nx; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[x], j & 1));
+    uint32_t s_count = 0, o_count = 0;
+    Reader reader;
+    Item it;
+    while (reader.next(bars, scratch, it) && it.n >= 0) {
+      const bool in = used && i < it.valid;
+      // Rows of no query compute on whatever is there and are not stored.
+      const int seen = in && p.causal ? clamp_index((int64_t)it.base + i, 0, it.lk) : it.lk;
+      const int nx = x ? it.n_b : it.n_a;
+      float m = kLowest, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < nx; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[x], s_count & 1));
+        if (!ok) break;
+        ++s_count;
+        tc_fence_after_sync();
+        softmax_step<T, HD>(s_tmem, o_tmem, seen - (it.lo + j) * BN, j > 0, scale2, m, l, &bars->p_half[x],
+                            &bars->p_full[x]);
+      }
+      if (ok && nx > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[x], o_count & 1));
+        ++o_count;
+        tc_fence_after_sync();
+      }
       if (!ok) {
         if (lane == 0) report_status(status, kFailSoftmax | 1);
         break;
       }
-      tc_fence_after_sync();
-      softmax_step<T, HD>(s_tmem, o_tmem, seen - (lo + j) * BN, j > 0, scale2, m, l, &bars->p_half[x],
-                          &bars->p_full[x]);
-    }
-    if (ok && n > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_final, 0));
-      if (!ok && lane == 0) report_status(status, kFailSoftmax | 2);
-      tc_fence_after_sync();
-    }
-    if (ok) {
       const long long place =
-          in ? (long long)(r.q0 + i) * p.o_tok + (long long)(hk * group + row % group) * p.o_head : -1;
+          in ? (long long)(it.row + i) * p.o_tok + (long long)(it.hk * group + row % group) * p.o_head : -1;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const long long slot = item * parts + part;
+      const long long slot = (long long)it.index * parts + it.part;
       const int slots = (int)gridDim.x;
       if (parts > 1) {
-        if (part == 0) reinterpret_cast<long long*>(p.work + tile_places_at())[item * kTileRows + x * 128 + row] = place;
+        if (it.part == 0)
+          reinterpret_cast<long long*>(p.work + tile_places_at())[(long long)it.index * kTileRows + x * 128 + row] = place;
         reinterpret_cast<float2*>(p.work + tile_stats_at(slots))[slot * kTileRows + x * 128 + row] = make_float2(m, l);
       }
       float* part_row = reinterpret_cast<float*>(p.work + tile_rows_at(slots)) + (slot * kTileRows + x * 128 + row) * HD;

@@ -369,8 +369,11 @@ class BoundRequest:
 
     def __del__(self):
         held, self._held = getattr(self, "_held", []), []
-        for ptr in held:
-            N.lib().tb_buffer_release(ptr)
+        try:
+            for ptr in held:
+                N.lib().tb_buffer_release(ptr)
+        except Exception:
+            pass
 
 
 def fill_normal(count: int, seed: int, mean: float = 0.0, std: float = 1.0, dtype: DType = DType.F32,
