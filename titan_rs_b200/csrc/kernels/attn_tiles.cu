@@ -51,6 +51,7 @@ static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kTileThreads * kTileLau
 constexpr int kSlots = 4;         // item descriptions in flight
 constexpr int kItemReaders = 11;  // warps 0, 1, 2 and the eight softmax warps
 constexpr int kQ = 3;             // Q tiles in shared memory
+constexpr long long kGroupBytes = 32ll << 20;  // K and V that are worked on at a time
 
 struct Barriers {
   uint64_t q_full[kQ], q_empty[kQ];
@@ -84,6 +85,20 @@ struct Scratch {
   long long scan[kTileThreads / 32];
 };
 static_assert(sizeof(Scratch) <= kTileScratchBytes, "scratch block overflows its reservation");
+
+// True in one lane of the warp (the same one each time), all of which call it. The compiler
+// knows of an elected lane that it is one: under `lane == 0` every tcgen05.mma was wrapped in
+// a loop over the lanes that might be there (eight prompts of 4096 tokens, 32 heads: 1194 us
+// against 1028).
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float x, float y);
@@ -127,6 +142,20 @@ __device__ __forceinline__ void exp_chunk(const uint32_t (&cur)[32], float2 scal
     packed[i / 2] = pack2<T>(e.x, e.y);
   }
   tmem_st_x16(p_tmem, packed);
+}
+
+// 32 bytes of a row, in one store where the rows are aligned to it. (A lane stores its own
+// row. Turning the rows of four lanes by shuffles, so that a store covers whole lines, cost
+// more issue slots than it saved: 261 against 243 us for 128 requests of 256 tokens, 32 heads.)
+__device__ __forceinline__ void store32(void* to, const uint32_t* r, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(to)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    reinterpret_cast<uint4*>(to)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+  }
 }
 
 template <int HD>
@@ -194,20 +223,42 @@ __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, i
   if (lane == 0) mbar_arrive(p_full);
 }
 
-template <int N>
-struct Int {
-  static constexpr int value = N;
-};
+// A wait that sleeps between polls, for the warps beside the pipeline: they share issue slots
+// with softmax warps (2% of a long prompt's time with mbar_wait in their place).
+__device__ __forceinline__ bool wait_idle(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  if (mbar_try_wait(at, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  for (uint32_t polls = 1; !mbar_try_wait(at, parity); ++polls) {
+    __nanosleep(300);
+    if (polls % 64 == 0 && global_timer_ns() - start > kWaitLimitNs) return false;
+  }
+  return true;
+}
 
 // A warp's place in the list of items: it reads each description and lets go of its slot.
 struct Reader {
   int slot = 0;
   uint32_t phase = 0;
 
+  // The next item's description, held until done(); null when the wait ran out. All lanes.
+  __device__ __forceinline__ const Item* hold(Barriers* bars, const Scratch* scratch) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars->item_full[slot], phase))) return nullptr;
+    return &scratch->items[slot];
+  }
+  __device__ __forceinline__ void done(Barriers* bars) {
+    __syncwarp();
+    if (lane_id() == 0) mbar_arrive(&bars->item_empty[slot]);
+    if (++slot == kSlots) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+
   // Called by all lanes of the warp, or (kLanes = 1) by one; false when the wait ran out.
-  template <int kLanes = 32>
+  template <int kLanes = 32, bool kIdle = false>
   __device__ __forceinline__ bool next(Barriers* bars, const Scratch* scratch, Item& item) {
-    bool ok = mbar_wait(&bars->item_full[slot], phase);
+    bool ok = kIdle ? wait_idle(&bars->item_full[slot], phase) : mbar_wait(&bars->item_full[slot], phase);
     if (kLanes > 1) ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       item = scratch->items[slot];
@@ -290,8 +341,8 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         const int slot = k % kSlots;
         // An item is drawn only when its predecessor nears its end, so no CTA sits on work that
         // another could begin.
-        if (!__all_sync(0xffffffffu, (k == 0 || mbar_wait(&bars->item_want, (k - 1) & 1)) &&
-                                         mbar_wait(&bars->item_empty[slot], ((k / kSlots) & 1) ^ 1))) {
+        if (!__all_sync(0xffffffffu, (k == 0 || wait_idle(&bars->item_want, (k - 1) & 1)) &&
+                                         wait_idle(&bars->item_empty[slot], ((k / kSlots) & 1) ^ 1))) {
           if (lane == 0) report_status(status, kFailSchedule | 1);
           break;
         }
@@ -303,7 +354,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         Item it{};
         it.n = -1;
         if (more) {
-          const long long index = w / parts, unit = stretch.total - 1 - index / p.kv_heads;
+          const long long index = w / parts, place = stretch.total * p.kv_heads - 1 - index, unit = place / p.kv_heads;
           const int part = (int)(w % parts);
           // Back over the requests, 32 at a time, to the one that holds `unit`.
           while (unit < before) {
@@ -321,7 +372,15 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
             b -= at + 1;
           }
           const AttnRequest r = request_of(p, b);
-          const int tok0 = (int)(unit - before) * 2 * p.tile_tokens;
+          // Inside a request: groups of key heads whose K and V stay in L2 while the group
+          // runs, and in a group the last pairs (with the most keys) of all its heads first.
+          const int pairs = pairs_of(p, r);
+          const long long turn = (before + pairs) * p.kv_heads - 1 - place;
+          const int heads_at_once = (int)min((long long)p.kv_heads, max(1ll, kGroupBytes / (4ll * HD * max(r.lk, 1))));
+          const long long in_group = (long long)heads_at_once * pairs;
+          const int first_head = (int)(turn / in_group) * heads_at_once;
+          const int rest = (int)(turn % in_group), heads = min(heads_at_once, p.kv_heads - first_head);
+          const int tok0 = (pairs - 1 - rest / heads) * 2 * p.tile_tokens;
           const bool has_b = tok0 + p.tile_tokens < r.lq;
           // Key tiles that each tile needs (of its last row), and this part's range of them.
           const int end_a = (visible_keys(p, r, min(tok0 + p.tile_tokens, r.lq) - 1) + BN - 1) / BN;
@@ -333,7 +392,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           it.n_a = max(0, min(hi, end_a) - lo);
           it.n_b = max(0, min(hi, end_b) - lo);
           it.lo = lo;
-          it.hk = (int)(index % p.kv_heads);
+          it.hk = first_head + rest % heads;
           it.b = b;
           it.row = r.q0 + tok0;
           it.valid = r.lq - tok0;
@@ -382,14 +441,6 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         for (int h = 0; h < S::kHalves; ++h)
           tma_load_4d(smem + off + h * S::kHalfBytes + lane * box * 128, map, bar, 64 * h, hk, row, w);
       };
-      const auto prefetch = [&](const Item& it, int j, int w) {
-        if (!active || j >= it.lo + it.n || (paged && w == p.pages)) return;
-#pragma unroll
-        for (int h = 0; h < S::kHalves; ++h) {
-          tma_prefetch_l2_4d(&tmap_k, 64 * h, it.hk, row_of(it, j), w);
-          tma_prefetch_l2_4d(&tmap_v, 64 * h, it.hk, row_of(it, j), w);
-        }
-      };
       int q_slot = 0;
       uint32_t q_phase = 1;  // of q_empty: the first round finds the slots free
       uint32_t q_issued[kQ] = {0, 0, 0}, kv_issued[2] = {0, 0};
@@ -431,7 +482,6 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         if (has_k) {
           if (lane == 0 && j == max(0, cur.n - 3)) mbar_arrive(&bars->item_want);
           w_after = page_at(cur, cur.lo + j + 2);
-          prefetch(cur, cur.lo + j + 1, w_next);
           if (j == 0 && cur.n_a > 0) ok = load_q(cur, 0);
           if (j + 1 == cur.n && ok) {
             // The item behind it, and its first pages, while this step's stage is still in use.
@@ -492,7 +542,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       // Step t: the products P V of the key tile before, then the scores Q K^T of this one,
       // per query tile. The step that begins an item ends the one before it, unless that has
       // no keys (or there is none): then a step without scores comes between.
-      if (lane == 0) {
+      if (elected()) {
         Reader reader;
         Item it{};
         bool ok = true, owed = false;
@@ -501,8 +551,9 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         const uint64_t qd0 = sdesc_sw128(smem_addr(smem + OFF_Q), 16, 1024);
         const uint64_t kd0 = sdesc_sw128(smem_addr(smem + OFF_K), 16, 1024);
         const uint64_t vd0 = sdesc_sw128(smem_addr(smem + OFF_V), S::kHalfBytes, 1024);
-        int q_a = 0, q_b = 0, q_slot = 0;
-        uint32_t q_phase = 0, step = 0, s_a = 0, s_b = 0;
+        int q_slot = 0, q_ab = 0;                     // the next Q slot; those of tiles A (low byte) and B
+        uint32_t q_phase = 0, step = 0, parities = 0;  // bit x: parity of tile x's next scores
+        uint32_t failed = 0;
         while (ok) {
           if (n <= 0 && !owed) {
             if (n < 0) break;
@@ -515,42 +566,37 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           const int st = step & 1;
           const uint64_t kd = desc_add(kd0, st * (S::kTileBytes >> 4));
           const uint64_t vd = desc_add(vd0, st * (S::kTileBytes >> 4));
-          if (!mbar_wait(&bars->kv_full[st], (step >> 1) & 1)) {
-            report_status(status, kFailMma | 2);
-            ok = false;
-            break;
-          }
-          const auto tile = [&](auto which, int nx, int pnx, int& q_at, uint32_t& scores) {
-            constexpr int x = decltype(which)::value;
+          if (!mbar_wait(&bars->kv_full[st], (step >> 1) & 1)) failed = 2;
+          // (Not unrolled, here and below: the roles' code competes for the instruction caches.
+          // Two copies of this body, and a third for steps inside an item, took 243 -> 310 us
+          // for 128 requests of 256 tokens.)
+#pragma unroll 1
+          for (int x = 0; x < 2 && !failed; ++x) {
+            const int nx = x ? n_b : n_a, pnx = x ? pn_b : pn_a;
             const uint32_t s_tmem = tmem + x * BN, o_tmem = tmem + (2 + x) * BN;
             if (pj < pnx) {
-              const uint32_t parity = (scores - 1) & 1;
+              const uint32_t parity = ((parities >> x) & 1) ^ 1;  // of the scores before
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                if (!mbar_wait(half ? &bars->p_full[x] : &bars->p_half[x], parity)) {
-                  report_status(status, kFailMma | 3);
-                  return false;
-                }
+                if (!mbar_wait(half ? &bars->p_full[x] : &bars->p_half[x], parity)) failed = 3;
                 tc_fence_after_sync();
 #pragma unroll
-                for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  umma_bf16_ts(o_tmem, s_tmem + k * 8, desc_add(vd, k * (2048 >> 4)), S::kIdescO,
-                               (k > 0 || pj > 0) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k)
+                  umma_bf16_ts(o_tmem, s_tmem + half * 32 + k * 8, desc_add(vd, half * 4 * (2048 >> 4) + k * (2048 >> 4)),
+                               S::kIdescO, (k + half > 0 || pj > 0) ? 1u : 0u);
               }
               if (pj + 1 == pnx) umma_commit(&bars->o_full[x]);
             }
             if (j < nx) {
               if (j == 0) {
-                if (!mbar_wait(&bars->q_full[q_slot], q_phase)) {
-                  report_status(status, kFailMma | 1);
-                  return false;
-                }
-                q_at = q_slot;
+                if (!mbar_wait(&bars->q_full[q_slot], q_phase)) failed = 1;
+                q_ab = x ? (q_ab & 0xff) | q_slot << 8 : (q_ab & ~0xff) | q_slot;
                 if (++q_slot == kQ) {
                   q_slot = 0;
                   q_phase ^= 1;
                 }
               }
+              const int q_at = (q_ab >> (8 * x)) & 0xff;
               const uint64_t qd = desc_add(qd0, q_at * (S::kTileBytes >> 4));
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k) {
@@ -558,13 +604,14 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
                 umma_bf16_ss(s_tmem, desc_add(qd, off), desc_add(kd, off), S::kIdescS, k > 0 ? 1u : 0u);
               }
               umma_commit(&bars->s_full[x]);
-              ++scores;
+              parities ^= 1u << x;
               if (j + 1 == nx) umma_commit(&bars->q_empty[q_at]);
             }
-            return true;
-          };
-          ok = tile(Int<0>(), n_a, pn_a, q_a, s_a) && tile(Int<1>(), n_b, pn_b, q_b, s_b);
-          if (!ok) break;
+          }
+          if (failed) {
+            report_status(status, kFailMma | failed);
+            break;
+          }
           umma_commit(&bars->kv_empty[st]);
           ++step;
           owed = n > 0;
@@ -588,14 +635,14 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       Item it;
       uint32_t step = 0, cleared[2] = {0, 0};
       bool owed = false;
-      while (reader.next(bars, scratch, it) && it.n >= 0) {
+      while (reader.next<32, true>(bars, scratch, it) && it.n >= 0) {
         if (it.n == 0 && owed) ++step;  // the step without scores
         owed = it.n > 0;
         step += it.n;
         if (it.last_rows == 0) continue;
         // Its V tile comes with the step behind the item's last key tile.
         const int st = step & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_raw[st], (st ? cleared[1] : cleared[0]) & 1))) {
+        if (!__all_sync(0xffffffffu, wait_idle(&bars->v_raw[st], (st ? cleared[1] : cleared[0]) & 1))) {
           if (lane == 0) report_status(status, kFailClear | 1);
           break;
         }
@@ -623,23 +670,31 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     const int i = x * p.tile_tokens + row / group;  // the query row, from tile A's first
     const bool used = row < p.tile_tokens * group;
     const float scale2 = p.scale * 1.4426950408889634f;
+    const bool wide = ((p.o | (uint64_t)(2 * (p.o_tok | p.o_head))) & 31) == 0;
     uint32_t s_count = 0, o_count = 0;
     Reader reader;
-    Item it;
-    while (reader.next(bars, scratch, it) && it.n >= 0) {
-      const bool in = used && i < it.valid;
+    for (;;) {
+      const Item* it = reader.hold(bars, scratch);
+      if (!it) {
+        if (lane == 0) report_status(status, kFailSoftmax | 2);
+        break;
+      }
+      if (it->n < 0) {
+        reader.done(bars);
+        break;
+      }
       // Rows of no query compute on whatever is there and are not stored.
-      const int seen = in && p.causal ? clamp_index((int64_t)it.base + i, 0, it.lk) : it.lk;
-      const int nx = x ? it.n_b : it.n_a;
+      const int seen = p.causal && used && i < it->valid ? clamp_index((int64_t)it->base + i, 0, it->lk) : it->lk;
+      const int nx = x ? it->n_b : it->n_a;
+      int valid = seen - it->lo * BN;
       float m = kLowest, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < nx; ++j) {
+      for (int j = 0; j < nx; ++j, valid -= BN) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[x], s_count & 1));
         if (!ok) break;
         ++s_count;
         tc_fence_after_sync();
-        softmax_step<T, HD>(s_tmem, o_tmem, seen - (it.lo + j) * BN, j > 0, scale2, m, l, &bars->p_half[x],
-                            &bars->p_full[x]);
+        softmax_step<T, HD>(s_tmem, o_tmem, valid, j > 0, scale2, m, l, &bars->p_half[x], &bars->p_full[x]);
       }
       if (ok && nx > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[x], o_count & 1));
@@ -650,43 +705,46 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         if (lane == 0) report_status(status, kFailSoftmax | 1);
         break;
       }
-      const long long place =
-          in ? (long long)(it.row + i) * p.o_tok + (long long)(it.hk * group + row % group) * p.o_head : -1;
+      const long long place = used && i < it->valid ? (long long)(it->row + i) * p.o_tok +
+                                                          (long long)(it->hk * group + row % group) * p.o_head
+                                                    : -1;
+      const long long slot = (long long)it->index * parts + it->part, first = (long long)it->index * kTileRows;
+      const bool leader = it->part == 0;
+      reader.done(bars);
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const long long slot = (long long)it.index * parts + it.part;
       const int slots = (int)gridDim.x;
       if (parts > 1) {
-        if (it.part == 0)
-          reinterpret_cast<long long*>(p.work + tile_places_at())[(long long)it.index * kTileRows + x * 128 + row] = place;
+        if (leader) reinterpret_cast<long long*>(p.work + tile_places_at())[first + x * 128 + row] = place;
         reinterpret_cast<float2*>(p.work + tile_stats_at(slots))[slot * kTileRows + x * 128 + row] = make_float2(m, l);
       }
       float* part_row = reinterpret_cast<float*>(p.work + tile_rows_at(slots)) + (slot * kTileRows + x * 128 + row) * HD;
-#pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
+      // 64 columns at a time: 128 bytes of an output row, 256 of a part's.
+#pragma unroll
+      for (int c = 0; c < HD; c += 64) {
+        uint32_t o[2][32];
         if (nx > 0) {
-          tmem_ld_x32(o_tmem + c, o);
+          tmem_ld_x32(o_tmem + c, o[0]);
+          tmem_ld_x32(o_tmem + c + 32, o[1]);
           tmem_ld_wait();
-          reg_fence(o);
+          reg_fence(o[0]);
+          reg_fence(o[1]);
         } else {
 #pragma unroll
-          for (int q = 0; q < 32; ++q) o[q] = 0u;
+          for (int q = 0; q < 32; ++q) o[0][q] = o[1][q] = 0u;
         }
-        if (in && parts > 1) {
+        if (parts > 1) {
+          // (Rows of no query are written too: their slots are the item's own.)
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            reinterpret_cast<uint4*>(part_row + c)[q] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-        } else if (in) {
-          uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + place + c);
+          for (int k = 0; k < 8; ++k) store32(part_row + c + 8 * k, &o[k >> 2][8 * (k & 3)], true);
+        } else if (place >= 0) {
+          uint32_t w[32];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 w;
-            w.x = pack2<T>(__uint_as_float(o[8 * q + 0]) * inv, __uint_as_float(o[8 * q + 1]) * inv);
-            w.y = pack2<T>(__uint_as_float(o[8 * q + 2]) * inv, __uint_as_float(o[8 * q + 3]) * inv);
-            w.z = pack2<T>(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv);
-            w.w = pack2<T>(__uint_as_float(o[8 * q + 6]) * inv, __uint_as_float(o[8 * q + 7]) * inv);
-            to[q] = w;
+          for (int q = 0; q < 32; ++q) {
+            const uint32_t* from = &o[q >> 4][2 * (q & 15)];
+            w[q] = pack2<T>(__uint_as_float(from[0]) * inv, __uint_as_float(from[1]) * inv);
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) store32(reinterpret_cast<T*>(p.o) + place + c + 16 * k, &w[8 * k], wide);
         }
       }
     }
