@@ -166,28 +166,21 @@ tb_status launch_tiles(Session* s, Stream* st, AttnCall* c, uint64_t longest) {
   uint64_t grid = pairs * (uint64_t)p.kv_heads;
   if (grid > 0x3fffffffull) return contract("attention work list exceeds 2^30 items");
   p.max_items = (int32_t)grid;
-  // Keys are cut into parts where the items cannot fill half of the SMs and there are keys
-  // enough for two parts of two tiles.
+  // One CTA an SM, drawing items until there are no more. The kernel may cut long requests
+  // where two parts of the smallest size fit their keys.
   const uint64_t keys = p.table ? (uint64_t)p.width * p.page : (uint64_t)p.tk;
-  const uint64_t sms = (uint64_t)s->sm_count;
-  p.splits = grid * 2 <= sms ? (int32_t)std::min<uint64_t>(kTileMaxSplits, keys / 256) : 1;
-  grid = p.splits > 1 ? sms : std::min(grid, sms);  // one CTA an SM, drawing items until there are no more
+  p.cut = keys > 128 * kTileMinPart ? 1 : 0;
+  const uint64_t sms = (uint64_t)std::min(s->sm_count, kTileMaxCtas);
+  grid = std::min(p.cut ? grid * kTileMaxParts : grid, sms);
   CUdeviceptr work = 0;
-  const size_t bytes = p.splits > 1 ? tile_workspace_bytes((int)grid, p.dim) : 4ull * kTokenCounters;
+  const size_t bytes = p.cut ? tile_workspace_bytes(2 * (int)grid, p.dim) : kWorkFront;
   if ((rc = stream_workspace(s, st, bytes, &work))) return rc;
   p.work = work;
   CUdeviceptr status = s->status.device;
   void* params[] = {&p, &mq, &mk, &mv, &status};
   rc = launch_builtin(s, st, fn, (unsigned)grid, 1, 1, kTileThreads, (unsigned)tile_smem_bytes(p.dim), params,
                       entry.c_str());
-  if (rc || p.splits <= 1) return rc;
-  const std::string join = "attention_tiles_join_" + suffix;
-  if ((rc = builtin_function(s, "attn_tiles", join.c_str(), &fn))) return rc;
-  int slots = (int)grid;
-  void* join_params[] = {&p, &slots};
-  if ((rc = launch_builtin(s, st, fn, (unsigned)s->sm_count, 1, 1, 256, 0, join_params, join.c_str()))) return rc;
-  note_candidate(entry.c_str());
-  return TB_OK;
+  return rc;
 }
 
 // Decode kernel for the requests of at most p.token_rows (row, head) pairs per key head.
@@ -197,7 +190,7 @@ tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
   CUfunction fn = nullptr;
   tb_status rc = builtin_function(s, "attn_tokens", entry.c_str(), &fn);
   if (rc) return rc;
-  const int ctas = std::min(2 * s->sm_count, kTileNext);  // two resident on each SM
+  const int ctas = std::min(2 * s->sm_count, kTokenMaxCtas);  // two resident on each SM
   CUdeviceptr work = 0;
   if ((rc = stream_workspace(s, st, token_workspace_bytes(ctas, c->p.token_rows, c->p.dim), &work))) return rc;
   c->p.work = work;

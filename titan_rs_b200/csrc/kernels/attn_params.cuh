@@ -37,18 +37,24 @@ struct AttnParams {
   uint64_t work;           // workspace of the token and tile kernels
   int32_t tile_tokens;     // query rows of a 128-row tile, 128 / (heads / kv_heads)
   int32_t max_items;       // (pair of tiles, key head) items of sound index tensors at most
-  int32_t splits;          // the tile kernel cuts a pair's keys into at most this many parts; with
-                           // more than one, the workspace has room for gridDim.x of them
+  int32_t cut;             // whether the tile kernel may cut an item's keys into parts (the
+                           // workspace then has two slots for each CTA)
 };
 
-// Layout of the token kernel's workspace: a counter per CTA, at the same place for every form
-// of the kernel (it is zero between launches), then two partial results a CTA (its first
-// request may have begun in an earlier CTA, its last may go on in a later one), each
-// rows x (dim + 2) floats: O, then the row's maximum and sum.
-constexpr int kTokenCounters = 1024;  // the token kernel's CTAs, and two of the tile kernel
+// The front of every workspace holds counters that are zero between launches, at the same
+// place for every kernel and form: one per CTA of the token kernel; the tile kernel's next
+// work number and its count of finished CTAs; and the finished parts of each of its slots' two
+// tiles.
+constexpr int kTokenMaxCtas = 1022, kTileNext = 1022, kTileDone = 1023, kTileParts = 1024;
+constexpr int kTileMaxCtas = 512;
+constexpr uint64_t kWorkFront = 4ull * (kTileParts + 2 * 2 * kTileMaxCtas);
+
+// The token kernel's partial results, behind the counters: two a CTA (its first request may
+// have begun in an earlier CTA, its last may go on in a later one), each rows x (dim + 2)
+// floats: O, then the row's maximum and sum.
 TB_BOTH constexpr uint64_t token_slot_floats(int rows, int dim) { return (uint64_t)rows * (dim + 2); }
 TB_BOTH constexpr uint64_t token_workspace_bytes(int ctas, int rows, int dim) {
-  return 4ull * kTokenCounters + 2ull * ctas * token_slot_floats(rows, dim) * 4;
+  return kWorkFront + 2ull * ctas * token_slot_floats(rows, dim) * 4;
 }
 
 // The token kernel: keys of a tile, stages of its ring, and its shared memory (the ring, the
@@ -58,31 +64,24 @@ TB_BOTH constexpr int token_smem_bytes(int dim) {
   return kTokenStages * 2 * kTokenTile * dim * 2 + 2 * kTokenTile * 16 + 2 * 4 * 8 * 4 + 128 + 128;
 }
 
-// The tile kernel's workspace, behind the token kernel's counters: what the joining kernel
-// reads (the parts of an item, per row; where the row goes), then the partial results.
-//   head:   int32 {items, parts per item}
-//   places: int64 element offset of each row in the output, -1 for no row (items x 256)
-//   stats:  float2 {maximum, sum} (items x parts x 256)
-//   rows:   float [dim] (items x parts x 256)
-// `slots` (items x parts) is at most the SM count.
+// The tile kernel's workspace for the parts of items whose keys are cut, in slots of 256 rows,
+// behind the counters at the workspace's front:
+//   stats:  float2 {maximum, sum} (slots x 256)
+//   rows:   float [dim] (slots x 256)
+// A cut is made where a request's key tiles exceed the average work of a CTA, so there are at
+// most two slots a CTA.
 constexpr int kTileRows = 256;  // two tiles of 128 (query row, head) pairs
-TB_BOTH constexpr uint64_t tile_places_at() { return 4ull * kTokenCounters + 256; }
-TB_BOTH constexpr uint64_t tile_stats_at(int slots) { return tile_places_at() + 8ull * kTileRows * slots; }
-TB_BOTH constexpr uint64_t tile_rows_at(int slots) { return tile_stats_at(slots) + 8ull * kTileRows * slots; }
+TB_BOTH constexpr uint64_t tile_rows_at(int slots) { return kWorkFront + 8ull * kTileRows * slots; }
 TB_BOTH constexpr uint64_t tile_workspace_bytes(int slots, int dim) {
   return tile_rows_at(slots) + 4ull * kTileRows * slots * dim;
 }
-constexpr int kTileMaxSplits = 32;
+constexpr int kTileMaxParts = 32, kTileMinPart = 4;  // parts of an item; key tiles of a part
 constexpr int kTileThreads = 384, kTileLaunchRegs = 168;
-constexpr int kTileBarrierBytes = 256, kTileScratchBytes = 512;
+constexpr int kTileBarrierBytes = 512, kTileScratchBytes = 512;
 // Three Q tiles, two stages of a K and a V tile, barriers and item descriptions.
 TB_BOTH constexpr int tile_smem_bytes(int dim) {
   return 7 * 128 * dim * 2 + kTileBarrierBytes + kTileScratchBytes + 1024;
 }
-// The tile kernel's work counter and its count of finished CTAs, the last two of the counters
-// at the workspace's front.
-constexpr int kTileNext = kTokenCounters - 2, kTileDone = kTokenCounters - 1;
-
 // The index arithmetic is shared by the kernels and a host test of it.
 #ifdef __CUDACC__
 #define TB_INDEX_FN __device__ __forceinline__

@@ -10,8 +10,8 @@
 // (sdpa_pair_common.cuh): while the tensor core runs one tile's products, the other's
 // warpgroup exponentiates. Per CTA, three warpgroups:
 //   warp 0       producer: Q once, then K_j and V_{j-1} into stage j & 1 of a 2-stage ring. A
-//                packed key tile is one box; a paged one is 128 / page boxes, each lane copying
-//                the page whose id it looked up one tile ahead. A page id that names no page, and
+//                packed key tile is one box; a paged one is 128 / page boxes, whose page ids
+//                the lanes look up two tiles ahead. A page id that names no page, and
 //                pages past the request's end, are given a coordinate outside the map, which
 //                the copy fills with zeros.
 //   warp 1       owns the tensor memory S_A | S_B | O_A | O_B; one lane issues the MMAs.
@@ -20,8 +20,11 @@
 //                use: their probabilities are 0, but 0 x NaN is not. Scores of such keys are
 //                replaced before use.
 //   warps 4..11  softmax, one row a thread, warps 4-7 tile A, 8-11 tile B.
-// When the calls' items cannot fill the SMs, each item's keys are cut into `parts`, whose
-// unfinished (O, maximum, sum) go to the workspace; attention_tiles_join adds them up.
+//   warp 3       items: persistent CTAs draw them from a counter. Requests with more key tiles than
+//                a CTA's share of the whole call are cut along the keys into parts, drawn first;
+//                then come requests with more than half of a share, a quarter, and the rest,
+//                so that no long item starts when the others are done. The warpgroup that
+//                finishes a tile's last part adds the parts up, in their order.
 // Bound by the softmax and the single issuing lane beside the tensor core, as the square kernel.
 // Every wait is bounded; on a timeout the kernel records a code, drains and returns.
 #include <cuda_fp16.h>
@@ -63,6 +66,7 @@ struct Barriers {
   uint64_t v_raw[2];                 // per stage: a V tile whose rows past the end warp 2 clears
   uint64_t drain;
   uint64_t item_full[kSlots], item_empty[kSlots];
+  uint64_t part_stored[2], part_known[2];  // per query tile: a part is in the workspace; whether it was the last one
   uint64_t item_want;                // the producer nears its item's end: draw the next one
   uint32_t tmem_base;
 };
@@ -77,12 +81,17 @@ struct Item {
   int base;              // local row i sees base + i keys (causal)
   int lk, k0;            // keys of the request, and its first row of k (packed)
   int last_rows;         // rows of the last key tile if it runs past the request's end, else 0
-  int index, part;       // item number and part
+  int parts, part;       // parts that the item's keys are cut into, and which this is
+  int slot, stride;      // slot of part 0, and the slots from one part to the next
 };
+
+constexpr int kClasses = 4;  // of requests, by their number of key tiles: cut, long, middling, short
 
 struct Scratch {
   Item items[kSlots];
-  long long scan[kTileThreads / 32];
+  long long sums[kTileThreads / 32];
+  unsigned long long works[kClasses];
+  int last[2];  // whether a warpgroup finished its tile's last part
 };
 static_assert(sizeof(Scratch) <= kTileScratchBytes, "scratch block overflows its reservation");
 
@@ -127,6 +136,20 @@ struct Shape {
 // Pairs of tiles of one request (0 where the token kernel takes it).
 __device__ __forceinline__ int pairs_of(const AttnParams& p, const AttnRequest& r) {
   return is_token_request(p, r) ? 0 : (r.lq + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+}
+
+__device__ __forceinline__ int key_tiles(const AttnRequest& r) { return (r.lk + BN - 1) / BN; }
+
+// The class of a request: 0 is cut into parts, 1 to 3 are long, middling and short next to
+// a CTA's share. A cut costs a CTA about six key tiles' time (the parts' rows go through
+// memory), so it has to save more.
+__device__ __forceinline__ int class_of(const AttnParams& p, const AttnRequest& r, long long share) {
+  const int n = key_tiles(r);
+  return p.cut && n > share + share / 8 + 6 ? 0 : n > share ? 1 : 2 * n > share ? 1 : 4 * n > share ? 2 : 3;
+}
+
+__device__ __forceinline__ int parts_of(const AttnRequest& r, long long share) {
+  return (int)min((long long)kTileMaxParts, (key_tiles(r) + share - 1) / share);
 }
 
 // One 32-column chunk of S to probabilities in the values' type, and its part of the row sum.
@@ -273,6 +296,47 @@ struct Reader {
   }
 };
 
+// The parts of four rows' columns, added up in their order by one thread (rows at, at + step, ..;
+// neighbouring lanes take neighbouring columns): M = max m_i, O = sum 2^(m_i - M) O_i /
+// sum 2^(m_i - M) l_i. `store(row, four values)` takes what is done.
+template <int HD, typename Store>
+__device__ __forceinline__ void join_parts(const float2* stats, const float* rows, int slot0, int stride, int parts,
+                                           int at, int step, int end, int column, Store store) {
+  constexpr int kRowsAtOnce = 4;
+  const auto slot_of = [&](int i) { return (long long)(slot0 + i * stride) * kTileRows; };
+  float m[kRowsAtOnce], l[kRowsAtOnce];
+  float4 acc[kRowsAtOnce];
+#pragma unroll
+  for (int k = 0; k < kRowsAtOnce; ++k) {
+    m[k] = kLowest;
+    l[k] = 0.f;
+    acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+#pragma unroll
+    for (int k = 0; k < kRowsAtOnce; ++k) {
+      const int row = min(at + k * step, end - 1);
+      const float2 st = __ldcg(stats + slot_of(i) + row);
+      const float4 o = __ldcg(reinterpret_cast<const float4*>(rows + (slot_of(i) + row) * HD + column));
+      const float big = fmaxf(m[k], st.x);
+      const float f = exp2_mufu(m[k] - big), g = exp2_mufu(st.x - big);
+      m[k] = big;
+      l[k] = fmaf(l[k], f, st.y * g);
+      acc[k].x = fmaf(acc[k].x, f, o.x * g);
+      acc[k].y = fmaf(acc[k].y, f, o.y * g);
+      acc[k].z = fmaf(acc[k].z, f, o.z * g);
+      acc[k].w = fmaf(acc[k].w, f, o.w * g);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRowsAtOnce; ++k) {
+    const float inv = l[k] == 0.f ? 0.f : 1.0f / l[k];
+    if (at + k * step < end)
+      store(at + k * step, make_float4(acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv));
+  }
+}
+
 template <typename T, int HD>
 __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUtensorMap& tmap_q,
                                                 const CUtensorMap& tmap_k, const CUtensorMap& tmap_v,
@@ -301,6 +365,8 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       mbar_init(&bars->p_full[i], 4);
       mbar_init(&bars->o_full[i], 1);
       mbar_init(&bars->v_raw[i], 1);
+      mbar_init(&bars->part_stored[i], 4);
+      mbar_init(&bars->part_known[i], 1);
     }
     mbar_init(&bars->drain, 1);
     mbar_init(&bars->item_want, 1);
@@ -314,16 +380,26 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
-  const auto units = [&](int b) { return pairs_of(p, request_of(p, b)); };
-  const Stretch stretch = count_units<kTileThreads>(p.batch, scratch->scan, units);
-  // (More than max_items only where cu_seqlens counts rows twice; the rest is then left.)
-  const long long items = min(stretch.total * p.kv_heads, (long long)p.max_items);
-  // Parts of an item: as many as fill the SMs, where the workspace has room for them.
-  const int parts = p.splits > 1 && items > 0 ? (int)max(1ll, min((long long)p.splits, gridDim.x / items)) : 1;
-  if (p.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) {
-    int* head = counters + kTokenCounters;
-    head[0] = parts > 1 ? (int)items : 0;
-    head[1] = parts;
+  // ---- a CTA's share of the call, in key tiles, and the works (parts of items) of each class ----
+  if (threadIdx.x < kClasses) scratch->works[threadIdx.x] = 0;
+  long long mine = 0;
+  for (int b = threadIdx.x; b < p.batch; b += kTileThreads) {
+    const AttnRequest r = request_of(p, b);
+    mine += (long long)pairs_of(p, r) * key_tiles(r);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+  if (lane == 0) scratch->sums[warp] = mine;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kTileThreads / 32; ++w) total += scratch->sums[w];
+  const long long share = max((long long)kTileMinPart, (total * p.kv_heads + gridDim.x - 1) / gridDim.x);
+  for (int b = threadIdx.x; b < p.batch; b += kTileThreads) {
+    const AttnRequest r = request_of(p, b);
+    const int c = class_of(p, r, share);
+    const int n = pairs_of(p, r) * (c == 0 ? parts_of(r, share) : 1);
+    if (n) atomicAdd(&scratch->works[c], (unsigned long long)n);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -334,9 +410,10 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     setmaxnreg_dec<kControlRegs>();
     if (warp == 3) {
       // ---------------- items: the longest rows first, drawn from a counter ----------------
-      long long w = blockIdx.x;
-      int b = p.batch;                   // the walk stands before request b,
-      long long before = stretch.total;  // which has this many units before it
+      long long w = blockIdx.x, class_end = 0, before = 0;  // works up to the class's end; units before request b
+      int c = -1, b = 0;                                     // the walk stands in class c before request b
+      // (More than max_items only where cu_seqlens counts rows twice; the rest is then left.)
+      const long long most = (long long)p.max_items + 2ll * gridDim.x;
       for (int k = 0;; ++k) {
         const int slot = k % kSlots;
         // An item is drawn only when its predecessor nears its end, so no CTA sits on work that
@@ -350,12 +427,21 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           if (lane == 0) w = (long long)gridDim.x + atomicAdd(counters + kTileNext, 1);
           w = __shfl_sync(0xffffffffu, w, 0);
         }
-        const bool more = w < items * parts;
+        while (c + 1 < kClasses && w >= class_end) {
+          class_end += (long long)scratch->works[++c] * p.kv_heads;
+          b = p.batch;
+          before = (long long)scratch->works[c];
+        }
+        const bool more = w < class_end && w < most;
         Item it{};
         it.n = -1;
         if (more) {
-          const long long index = w / parts, place = stretch.total * p.kv_heads - 1 - index, unit = place / p.kv_heads;
-          const int part = (int)(w % parts);
+          // Units of the class, a pair of tiles or a part of one: the last request's come first.
+          const auto units = [&](int at) {
+            const AttnRequest r = request_of(p, at);
+            return class_of(p, r, share) == c ? pairs_of(p, r) * (c == 0 ? parts_of(r, share) : 1) : 0;
+          };
+          const long long place = class_end - 1 - w, unit = place / p.kv_heads;
           // Back over the requests, 32 at a time, to the one that holds `unit`.
           while (unit < before) {
             const int mine = b - 1 - lane;
@@ -374,13 +460,14 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           const AttnRequest r = request_of(p, b);
           // Inside a request: groups of key heads whose K and V stay in L2 while the group
           // runs, and in a group the last pairs (with the most keys) of all its heads first.
-          const int pairs = pairs_of(p, r);
-          const long long turn = (before + pairs) * p.kv_heads - 1 - place;
+          const int pairs = pairs_of(p, r), parts = c == 0 ? parts_of(r, share) : 1;
+          const long long turn = (before + (long long)pairs * parts) * p.kv_heads - 1 - place;
           const int heads_at_once = (int)min((long long)p.kv_heads, max(1ll, kGroupBytes / (4ll * HD * max(r.lk, 1))));
-          const long long in_group = (long long)heads_at_once * pairs;
+          const long long in_group = (long long)heads_at_once * pairs * parts;
           const int first_head = (int)(turn / in_group) * heads_at_once;
           const int rest = (int)(turn % in_group), heads = min(heads_at_once, p.kv_heads - first_head);
-          const int tok0 = (pairs - 1 - rest / heads) * 2 * p.tile_tokens;
+          const int tok0 = (pairs - 1 - rest / (heads * parts)) * 2 * p.tile_tokens;
+          const int part = rest % (heads * parts) / heads;
           const bool has_b = tok0 + p.tile_tokens < r.lq;
           // Key tiles that each tile needs (of its last row), and this part's range of them.
           const int end_a = (visible_keys(p, r, min(tok0 + p.tile_tokens, r.lq) - 1) + BN - 1) / BN;
@@ -392,7 +479,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           it.n_a = max(0, min(hi, end_a) - lo);
           it.n_b = max(0, min(hi, end_b) - lo);
           it.lo = lo;
-          it.hk = first_head + rest % heads;
+          it.hk = first_head + rest % (heads * parts) % heads;
           it.b = b;
           it.row = r.q0 + tok0;
           it.valid = r.lq - tok0;
@@ -400,8 +487,10 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           it.lk = r.lk;
           it.k0 = r.k0;
           it.last_rows = it.n > 0 && hi == r.lk / BN + 1 ? r.lk % BN : 0;
-          it.index = (int)index;
+          it.parts = parts;
           it.part = part;
+          it.slot = c == 0 ? (int)(w - (long long)part * heads) : 0;
+          it.stride = heads;
         }
         if (lane == 0) {
           scratch->items[slot] = it;
@@ -436,10 +525,15 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         return id < 0 ? p.pages : id;
       };
       const auto load = [&](int off, const CUtensorMap* map, uint64_t* bar, int hk, int row, int w) {
-        if (!active) return;
+#pragma unroll 1
+        for (int i = 0; i < boxes; ++i) {
+          const int page = __shfl_sync(0xffffffffu, w, i);
+          if (elected()) {
 #pragma unroll
-        for (int h = 0; h < S::kHalves; ++h)
-          tma_load_4d(smem + off + h * S::kHalfBytes + lane * box * 128, map, bar, 64 * h, hk, row, w);
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_load_4d(smem + off + h * S::kHalfBytes + i * box * 128, map, bar, 64 * h, hk, row, page);
+          }
+        }
       };
       int q_slot = 0;
       uint32_t q_phase = 1;  // of q_empty: the first round finds the slots free
@@ -667,11 +761,11 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + lane_off + x * BN;
     const uint32_t o_tmem = tmem + lane_off + (2 + x) * BN;
-    const int i = x * p.tile_tokens + row / group;  // the query row, from tile A's first
+    const int i = x * p.tile_tokens + row / group, head = row % group;  // the query row, from tile A's first
     const bool used = row < p.tile_tokens * group;
     const float scale2 = p.scale * 1.4426950408889634f;
     const bool wide = ((p.o | (uint64_t)(2 * (p.o_tok | p.o_head))) & 31) == 0;
-    uint32_t s_count = 0, o_count = 0;
+    uint32_t s_count = 0, o_count = 0, part_count = 0;
     Reader reader;
     for (;;) {
       const Item* it = reader.hold(bars, scratch);
@@ -705,47 +799,85 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         if (lane == 0) report_status(status, kFailSoftmax | 1);
         break;
       }
-      const long long place = used && i < it->valid ? (long long)(it->row + i) * p.o_tok +
-                                                          (long long)(it->hk * group + row % group) * p.o_head
-                                                    : -1;
-      const long long slot = (long long)it->index * parts + it->part, first = (long long)it->index * kTileRows;
-      const bool leader = it->part == 0;
-      reader.done(bars);
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const int slots = (int)gridDim.x;
-      if (parts > 1) {
-        if (leader) reinterpret_cast<long long*>(p.work + tile_places_at())[first + x * 128 + row] = place;
-        reinterpret_cast<float2*>(p.work + tile_stats_at(slots))[slot * kTileRows + x * 128 + row] = make_float2(m, l);
-      }
-      float* part_row = reinterpret_cast<float*>(p.work + tile_rows_at(slots)) + (slot * kTileRows + x * 128 + row) * HD;
-      // 64 columns at a time: 128 bytes of an output row, 256 of a part's.
-#pragma unroll
-      for (int c = 0; c < HD; c += 64) {
-        uint32_t o[2][32];
+      const bool in = used && i < it->valid;
+      const int first = it->row, head0 = it->hk * group;
+      if (it->parts == 1) {
+        reader.done(bars);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        uint32_t o[HD];
         if (nx > 0) {
-          tmem_ld_x32(o_tmem + c, o[0]);
-          tmem_ld_x32(o_tmem + c + 32, o[1]);
+#pragma unroll
+          for (int c = 0; c < HD; c += 32) tmem_ld_x32(o_tmem + c, reinterpret_cast<uint32_t(&)[32]>(o[c]));
           tmem_ld_wait();
-          reg_fence(o[0]);
-          reg_fence(o[1]);
+          reg_fence(o);
         } else {
 #pragma unroll
-          for (int q = 0; q < 32; ++q) o[0][q] = o[1][q] = 0u;
+          for (int c = 0; c < HD; ++c) o[c] = 0u;
         }
-        if (parts > 1) {
-          // (Rows of no query are written too: their slots are the item's own.)
+        if (in) {
+          T* to = reinterpret_cast<T*>(p.o) + (first + i) * p.o_tok + (head0 + head) * p.o_head;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) store32(part_row + c + 8 * k, &o[k >> 2][8 * (k & 3)], true);
-        } else if (place >= 0) {
-          uint32_t w[32];
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t w[8];
 #pragma unroll
-          for (int q = 0; q < 32; ++q) {
-            const uint32_t* from = &o[q >> 4][2 * (q & 15)];
-            w[q] = pack2<T>(__uint_as_float(from[0]) * inv, __uint_as_float(from[1]) * inv);
+            for (int q = 0; q < 8; ++q)
+              w[q] = pack2<T>(__uint_as_float(o[c + 2 * q]) * inv, __uint_as_float(o[c + 2 * q + 1]) * inv);
+            store32(to + c, w, wide);
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) store32(reinterpret_cast<T*>(p.o) + place + c + 16 * k, &w[8 * k], wide);
         }
+        continue;
+      }
+      // ---- a part: its rows go to the workspace, and who brings the last part joins them ----
+      const int parts = it->parts, slot0 = it->slot, stride = it->stride;
+      const long long own = (long long)(slot0 + it->part * stride) * kTileRows;
+      const int rows = min(p.tile_tokens, it->valid - x * p.tile_tokens) * group;
+      reader.done(bars);
+      float2* const stats = reinterpret_cast<float2*>(p.work + kWorkFront) + x * 128;
+      float* const parts_o = reinterpret_cast<float*>(p.work + tile_rows_at(2 * gridDim.x)) + (long long)x * 128 * HD;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (nx > 0) {
+          tmem_ld_x32(o_tmem + c, o);
+          tmem_ld_wait();
+          reg_fence(o);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) o[q] = 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store32(parts_o + (own + row) * HD + c + 8 * k, &o[8 * k], true);
+      }
+      stats[own + row] = make_float2(m, l);
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->part_stored[x]);
+      if (quarter == 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->part_stored[x], part_count & 1));
+        if (ok && lane == 0) {
+          int* counter = reinterpret_cast<int*>(p.work) + kTileParts + 2 * slot0 + x;
+          const bool last = atomicAdd(counter, 1) == parts - 1;
+          if (last) *counter = 0;  // as the next launch finds it
+          scratch->last[x] = last;
+          mbar_arrive(&bars->part_known[x]);
+        }
+      }
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars->part_known[x], part_count & 1));
+      if (!ok) {
+        if (lane == 0) report_status(status, kFailSoftmax | 3);
+        break;
+      }
+      ++part_count;
+      if (scratch->last[x]) {
+        __threadfence();
+        constexpr int kLanes = HD / 4, kStep = 128 / kLanes;  // lanes of a row, rows at a time
+        const int column = row % kLanes * 4;
+        for (int at = row / kLanes; at < rows; at += 4 * kStep)
+          join_parts<HD>(stats, parts_o, slot0, stride, parts, at, kStep, rows, column, [&](int r, float4 v) {
+            *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + (first + x * p.tile_tokens + r / group) * p.o_tok +
+                                      (head0 + r % group) * p.o_head + column) =
+                make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+          });
       }
     }
   }
@@ -759,41 +891,6 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
   }
 }
 
-// Adds up the parts of every row, one warp a row: M = max m_i, O = sum 2^(m_i - M) O_i /
-// sum 2^(m_i - M) l_i. Leaves at once when the call was not split.
-template <typename T, int HD>
-__device__ __forceinline__ void join_tiles(const AttnParams& p, int slots) {
-  const int* head = reinterpret_cast<const int*>(p.work + 4ull * kTokenCounters);
-  const long long rows = (long long)head[0] * kTileRows;
-  const int parts = head[1];
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = HD / 32;
-  for (long long u = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < rows;
-       u += (long long)gridDim.x * (blockDim.x >> 5)) {
-    const long long place = reinterpret_cast<const long long*>(p.work + tile_places_at())[u];
-    if (place < 0) continue;
-    const long long item = u / kTileRows, row = u % kTileRows;
-    float m = kLowest, l = 0.f, acc[kPer];
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      const long long at = (item * parts + i) * kTileRows + row;
-      const float2 st = reinterpret_cast<const float2*>(p.work + tile_stats_at(slots))[at];
-      const float* o = reinterpret_cast<const float*>(p.work + tile_rows_at(slots)) + at * HD + lane * kPer;
-      const float big = fmaxf(m, st.x);
-      const float f = exp2_mufu(m - big), g = exp2_mufu(st.x - big);
-      m = big;
-      l = l * f + st.y * g;
-#pragma unroll
-      for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * f + o[c] * g;
-    }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.o) + place + lane * kPer);
-#pragma unroll
-    for (int c = 0; c < kPer; c += 2) to[c / 2] = pack2<T>(acc[c] * inv, acc[c + 1] * inv);
-  }
-}
-
 }  // namespace
 
 // One CTA per SM at 168 registers a thread; the warpgroups re-divide them (56 and 216).
@@ -803,10 +900,6 @@ __device__ __forceinline__ void join_tiles(const AttnParams& p, int slots) {
                                const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, \
                                uint32_t* status) {                                                                  \
     attention_tiles<T, HD>(p, tmap_q, tmap_k, tmap_v, status);                                                      \
-  }                                                                                                                 \
-  extern "C" __global__ void __launch_bounds__(256) attention_tiles_join_##suffix(                                  \
-      const __grid_constant__ tb::AttnParams p, int slots) {                                                        \
-    join_tiles<T, HD>(p, slots);                                                                                    \
   }
 
 TB_TILE_ENTRY(bf16_d128, __nv_bfloat16, 128)

@@ -330,7 +330,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       const long long last = ((first_tile + cur.tiles) * ctas - 1) / total;
       const int parts = (int)(last - first + 1);
       const int rows = cur.r.lq * group;
-      float* slots = reinterpret_cast<float*>(p.work) + kTokenCounters;
+      float* slots = reinterpret_cast<float*>(p.work + kWorkFront);
       const uint64_t slot_floats = token_slot_floats(kRows, D);
       // The tile's stage is free until the next iteration's copies.
       float(*joined)[8][D + 4] = reinterpret_cast<float(*)[8][D + 4]>(sm.stage[n % kStages]);
