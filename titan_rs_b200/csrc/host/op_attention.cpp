@@ -214,11 +214,15 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
   std::lock_guard<std::mutex> lock(st->enqueue);
   const uint64_t group = (uint64_t)(c->p.heads / c->p.kv_heads);
   const uint64_t longest = a.max_query && a.max_query < (uint64_t)c->p.tq ? a.max_query : (uint64_t)c->p.tq;
-  if (c->p.table && !a.candidate && rows_aligned(c->p) && group <= 32) {
-    // Sized for every request where the caller's bound says so, for single tokens otherwise.
-    const uint64_t rows = longest * group <= 32 ? longest * group : group;
+  const bool tokens = c->p.table && !a.candidate && rows_aligned(c->p);
+  // A step whose requests all have few rows (the caller's bound says so) is the token kernel's.
+  // Other steps take one launch of the tile kernel, which reads single tokens' keys at 100 us
+  // for 64 requests of 300-8192 keys beside chunks (a launch of each kernel costs more).
+  const bool few = tokens && longest * group <= 32;
+  if (few || (tokens && !tiles && group <= 32)) {
+    const uint64_t rows = few ? longest * group : group;
     c->p.token_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-    if ((rc = launch_tokens(s, st, c)) || longest * group <= (uint64_t)c->p.token_rows) return rc;
+    if ((rc = launch_tokens(s, st, c)) || few) return rc;
   }
   return tiles ? launch_tiles(s, st, c, longest) : launch_rows(s, st, c);
 }
