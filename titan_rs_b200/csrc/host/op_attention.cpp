@@ -93,20 +93,19 @@ tb_status launch_rows(Session* s, Stream* st, AttnCall* c) {
   return launch_builtin(s, st, fn, (unsigned)grid, 1, 1, 256, 0, params, entry);
 }
 
-// Whether the tensor cores' 16-byte copies reach every row of K and V, and 4-byte loads every
-// row of Q.
+// Whether 16-byte copies reach every row of Q, K and V.
 bool rows_aligned(const AttnParams& p) {
   const uint64_t kv = p.k | p.v | (uint64_t)(2 * (p.k_tok | p.k_head | p.k_page | p.v_tok | p.v_head | p.v_page));
   const uint64_t q = p.q | (uint64_t)(2 * (p.q_tok | p.q_head));
-  return (p.dim == 64 || p.dim == 128) && (kv & 15) == 0 && (q & 3) == 0;
+  return (p.dim == 64 || p.dim == 128) && ((kv | q) & 15) == 0;
 }
 
-// Whether the tile kernel takes the call: 16-byte rows of Q and the output too, a group that
+// Whether the tile kernel takes the call: 16-byte rows of the output too, a group that
 // fits a tile, and pages that cut a 128-key tile evenly (or are cut by it).
 bool tiles_fit(const AttnParams& p) {
-  const uint64_t qo = p.q | p.o | (uint64_t)(2 * (p.q_tok | p.q_head | p.o_tok | p.o_head));
+  const uint64_t o = p.o | (uint64_t)(2 * (p.o_tok | p.o_head));
   const bool pages = !p.table || (p.page >= 8 && 128 % p.page == 0) || p.page % 128 == 0;
-  return rows_aligned(p) && (qo & 15) == 0 && p.heads / p.kv_heads <= 128 && pages;
+  return rows_aligned(p) && (o & 15) == 0 && p.heads / p.kv_heads <= 128 && pages;
 }
 
 // A map of rows of `dim` elements with up to three outer dimensions, copied in boxes of 64
@@ -195,7 +194,7 @@ tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
   if ((rc = stream_workspace(s, st, token_workspace_bytes(ctas, c->p.token_rows, c->p.dim), &work))) return rc;
   c->p.work = work;
   void* params[] = {&c->p};
-  return launch_builtin(s, st, fn, (unsigned)ctas, 1, 1, kTokenThreads, (unsigned)token_smem_bytes(c->p.dim), params,
+  return launch_builtin(s, st, fn, (unsigned)ctas, 1, 1, kTokenThreads, (unsigned)token_smem_bytes(c->p.dim, c->p.token_rows), params,
                         entry.c_str());
 }
 

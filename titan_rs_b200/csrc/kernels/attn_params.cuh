@@ -58,10 +58,12 @@ TB_BOTH constexpr uint64_t token_workspace_bytes(int ctas, int rows, int dim) {
 }
 
 // The token kernel: keys of a tile, stages of its ring, and its shared memory (the ring, the
-// row offsets of two tiles, the joined statistics and some words; 128 bytes to align).
+// row offsets of three tiles, two Q blocks where they fit (16 rows), the joined statistics
+// and some words; 128 bytes to align).
 constexpr int kTokenTile = 64, kTokenStages = 3, kTokenThreads = 128;
-TB_BOTH constexpr int token_smem_bytes(int dim) {
-  return kTokenStages * 2 * kTokenTile * dim * 2 + 2 * kTokenTile * 16 + 2 * 4 * 8 * 4 + 128 + 128;
+TB_BOTH constexpr int token_smem_bytes(int dim, int rows) {
+  return kTokenStages * (2 * kTokenTile * dim * 2 + kTokenTile * 16) + (rows <= 16 ? 2 * rows * dim * 2 : 0) +
+         2 * 4 * 8 * 4 + 256 + 128;
 }
 
 // The tile kernel's workspace for the parts of items whose keys are cut, in slots of 256 rows,

@@ -33,6 +33,7 @@ constexpr int kTile = kTokenTile;  // 16 keys a warp
 constexpr int kThreads = kTokenThreads;
 constexpr int kStages = kTokenStages;
 constexpr float kLowest = -3.402823466e38f;
+constexpr int kMinRun = 2;  // tiles of a CTA at least, where there are so many (11.3 us for 1018 keys x 8 heads; 12.5 with 1, 12.7 with 4)
 
 template <int D>
 TB_BOTH constexpr int stage_bytes() { return 2 * kTile * D * 2; }
@@ -74,7 +75,6 @@ struct Half<__nv_bfloat16> {
     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
 };
 template <>
 struct Half<__half> {
@@ -87,8 +87,29 @@ struct Half<__half> {
     const __half2 v = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
 };
+
+__device__ __forceinline__ void add_scaled(float4& a, const float4& v, float f) {
+  a.x = fmaf(v.x, f, a.x);
+  a.y = fmaf(v.y, f, a.y);
+  a.z = fmaf(v.z, f, a.z);
+  a.w = fmaf(v.w, f, a.w);
+}
+
+// Four elements of a finished row, O / sum (zeros where no key was seen).
+template <typename T>
+__device__ __forceinline__ void store_row4(T* to, const float4& o, float l) {
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const uint32_t lo = Half<T>::pack(o.x * inv, o.y * inv), hi = Half<T>::pack(o.z * inv, o.w * inv);
+  if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+  } else {  // a row that starts at an odd element
+    reinterpret_cast<uint16_t*>(to)[0] = (uint16_t)lo;
+    reinterpret_cast<uint16_t*>(to)[1] = (uint16_t)(lo >> 16);
+    reinterpret_cast<uint16_t*>(to)[2] = (uint16_t)hi;
+    reinterpret_cast<uint16_t*>(to)[3] = (uint16_t)(hi >> 16);
+  }
+}
 
 // Tiles of one (request, key head) pair; 0 for a request that is not this kernel's. A
 // request without keys has one empty tile, which writes its zeros.
@@ -119,20 +140,33 @@ struct Cursor {
   }
 };
 
-template <int D>
+// What a tile's copies need: where its rows lie, and, in a pair's first tile of the run, which
+// query rows come with it.
+struct TileRows {
+  long long k[kTile], v[kTile];  // element offsets, or -1 for a row of zeros
+};
+struct PairRows {
+  int q_row, rows, head;  // first row of q, (query row, head) pairs (0: not a first tile), key head
+};
+
+template <int D, int kRows>
 struct Shared {
   alignas(128) uint8_t stage[kStages][stage_bytes<D>()];  // K rows, then V rows; 16-byte chunks swizzled by row
-  long long k_at[2][kTile], v_at[2][kTile];  // element offsets of a tile's rows, or -1
+  alignas(16) uint8_t q[kRows <= 16 ? 2 : 0][kRows * D * 2 + (kRows <= 16 ? 0 : 16)];
+  TileRows at[kStages];
   float top[4][8], sum[4][8];
+  PairRows pair[kStages];
   long long scan[kThreads / 32], found_before;
   int found_b, last;
 };
 
 template <typename T, int D, int NT>
 __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
-  extern __shared__ uint8_t raw[];
-  Shared<D>& sm = *reinterpret_cast<Shared<D>*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
   constexpr int kRows = 8 * NT;
+  constexpr bool kQShared = kRows <= 16;  // Q comes through shared memory, else by plain loads
+  extern __shared__ uint8_t raw[];
+  using Smem = Shared<D, kRows>;
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
   constexpr int kChunks = D / 8;                    // 16-byte chunks of a row
   constexpr int kRowsAtOnce = kThreads / kChunks;   // rows one pass of the CTA copies
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -142,8 +176,8 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
   const auto units = [&](int b) { return tiles_of(p, request_of(p, b)); };
   const Stretch stretch = count_units<kThreads>(p.batch, sm.scan, units);
   const long long total = stretch.total * p.kv_heads;
-  const long long ctas = min((long long)gridDim.x, total);
-  if (blockIdx.x >= ctas) return;
+  const long long ctas = min((long long)gridDim.x, max(1ll, total / kMinRun));
+  if (blockIdx.x >= ctas || total == 0) return;
   const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
   // The tiles of a request start at kv_heads x (tiles before it).
   find_unit(stretch, begin / p.kv_heads, units, &sm.found_b, &sm.found_before);
@@ -161,7 +195,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
   auto look_up = [&](long long& k_off, long long& v_off) {
     const int j = ahead.tile * kTile + tid;
     k_off = v_off = -1;
-    if (j < ahead.r.lk) {
+    if (tid < kTile && j < ahead.r.lk) {
       const int id = page_of(p, ahead.b, j / p.page);
       if (id >= 0) {
         const int row = j % p.page;
@@ -170,31 +204,65 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       }
     }
   };
-  // Copies of tile n (its offsets are in shared memory) into its stage.
+  auto pair_of = [&](int n) {
+    return PairRows{ahead.r.q0, n == 0 || ahead.tile == 0 ? ahead.r.lq * group : 0, ahead.head};
+  };
+  auto publish = [&](int n, long long k_off, long long v_off, const PairRows& pair) {
+    if (tid < kTile) {
+      sm.at[n % kStages].k[tid] = k_off;
+      sm.at[n % kStages].v[tid] = v_off;
+    }
+    if (tid == kTile) sm.pair[n % kStages] = pair;
+  };
+  // Copies of tile n (its offsets are in shared memory) into its stage, and of the query rows
+  // of a pair that begins with it into the Q block that its number says.
   const int chunk = tid % kChunks, row0 = tid / kChunks;
+  int q_next = 0;
   auto copy_tile = [&](int n) {
     const uint32_t base = smem_of(sm.stage[n % kStages]);
+    const TileRows& rows = sm.at[n % kStages];
 #pragma unroll
     for (int r = row0; r < kTile; r += kRowsAtOnce) {
       const uint32_t at = base + r * (D * 2) + ((chunk ^ (r & 7)) << 4);
-      const long long k = sm.k_at[n & 1][r], v = sm.v_at[n & 1][r];
+      const long long k = rows.k[r], v = rows.v[r];
       copy16(at, reinterpret_cast<const T*>(p.k) + (k < 0 ? 0 : k) + chunk * 8, k >= 0);
       copy16(at + kTile * D * 2, reinterpret_cast<const T*>(p.v) + (v < 0 ? 0 : v) + chunk * 8, v >= 0);
     }
+    if constexpr (kQShared) {
+      const PairRows pair = sm.pair[n % kStages];
+      if (pair.rows) {
+        const uint32_t to = smem_of(sm.q[q_next]);
+        q_next ^= 1;
+#pragma unroll
+        for (int r = row0; r < kRows; r += kRowsAtOnce) {
+          const bool in = r < pair.rows;
+          const T* from = reinterpret_cast<const T*>(p.q) +
+                          (in ? (pair.q_row + r / group) * p.q_tok + (pair.head * group + r % group) * p.q_head : 0);
+          copy16(to + r * (D * 2) + ((chunk ^ (r & 7)) << 4), from + chunk * 8, in);
+        }
+      }
+    }
   };
 
-  // Two tiles' offsets are held: those of the tile that is copied next, and of the one behind it.
-  long long k_next = 0, v_next = 0;
-  for (int n = 0; n < kStages; ++n) {
-    if (n < count) {
-      if (tid < kTile) look_up(sm.k_at[n & 1][tid], sm.v_at[n & 1][tid]);
-      ahead.next(p);
+  long long k_next[kStages], v_next[kStages];
+  {
+    PairRows pairs[kStages];
+#pragma unroll
+    for (int n = 0; n < kStages; ++n) {
+      if (n < count) {
+        look_up(k_next[n], v_next[n]);
+        pairs[n] = pair_of(n);
+        ahead.next(p);
+      }
     }
-    if (n + 1 == kStages) break;  // copied in the first iteration
-    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < kStages; ++n)
+      if (n < count) publish(n, k_next[n], v_next[n], pairs[n]);
+  }
+  __syncthreads();
+  for (int n = 0; n < kStages - 1; ++n) {
     if (n < count) copy_tile(n);
     copies_commit();
-    __syncthreads();
   }
 
   uint32_t qf[NT][D / 16][2];  // Q^T fragments
@@ -203,9 +271,9 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
   int seen[NT][2];             // visible keys of the thread's query rows
   const float scale2 = p.scale * 1.4426950408889634f;
   bool fresh = true;
+  int q_now = 0;
   for (int n = 0; n < count; ++n) {
-    if (fresh) {
-      fresh = false;
+    if (!kQShared && fresh) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int row = t * 8 + (lane >> 2);
@@ -218,6 +286,33 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
           qf[t][k][0] = in ? __ldg(at) : 0u;
           qf[t][k][1] = in ? __ldg(at + 4) : 0u;
         }
+      }
+    }
+    copies_wait<kStages - 2>();
+    __syncthreads();  // tile n is here, and every warp is done with the stage of tile n - 1
+    if (fresh) {
+      if constexpr (kQShared) {
+        const uint32_t from = smem_of(sm.q[q_now]);
+        q_now ^= 1;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int r = t * 8 + (lane & 7);
+#pragma unroll
+          for (int k = 0; k < D / 16; k += 2) {  // two 16-dimension slices at a time
+            uint32_t a[4];
+            load_matrix(a, from + r * (D * 2) + (((k * 2 + (lane >> 3)) ^ (r & 7)) << 4));
+            qf[t][k][0] = a[0];
+            qf[t][k][1] = a[1];
+            qf[t][k + 1][0] = a[2];
+            qf[t][k + 1][1] = a[3];
+          }
+        }
+        // The block is read before the copies of the pair two behind this one, which may
+        // begin in this iteration.
+        __syncthreads();
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int r = t * 8 + (lane & 3) * 2 + i;
@@ -230,13 +325,16 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[t][k][i] = 0.f;
       }
+      fresh = false;
     }
-    copies_wait<kStages - 2>();
-    __syncthreads();  // tile n is here, and every warp is done with the stage of tile n - 1
     if (n + kStages - 1 < count) copy_tile(n + kStages - 1);
     copies_commit();
     const bool more = n + kStages < count;
-    if (more && tid < kTile) look_up(k_next, v_next);
+    PairRows pair{};
+    if (more) {
+      look_up(k_next[0], v_next[0]);
+      pair = pair_of(n + kStages);
+    }
 
     // ---- S^T of the warp's 16 keys ----
     const uint32_t ks = smem_of(sm.stage[n % kStages]) + warp * 16 * D * 2, vs = ks + kTile * D * 2;
@@ -316,10 +414,8 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       }
     }
     if (more) {
-      if (tid < kTile) {
-        sm.k_at[(n + kStages) & 1][tid] = k_next;
-        sm.v_at[(n + kStages) & 1][tid] = v_next;
-      }
+      // (Tile n's offsets were used two iterations ago.)
+      publish(n + kStages, k_next[0], v_next[0], pair);
       ahead.next(p);
     }
 
@@ -332,6 +428,8 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       const int rows = cur.r.lq * group;
       float* slots = reinterpret_cast<float*>(p.work + kWorkFront);
       const uint64_t slot_floats = token_slot_floats(kRows, D);
+      T* const out = reinterpret_cast<T*>(p.o) + cur.r.q0 * p.o_tok + cur.head * group * p.o_head;
+      const auto place = [&](int row) { return out + (row / group) * p.o_tok + (row % group) * p.o_head; };
       // The tile's stage is free until the next iteration's copies.
       float(*joined)[8][D + 4] = reinterpret_cast<float(*)[8][D + 4]>(sm.stage[n % kStages]);
       static_assert(sizeof(float) * 4 * 8 * (D + 4) <= stage_bytes<D>(), "joined results fit a stage");
@@ -360,28 +458,24 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         }
         __syncthreads();
         const int limit = min(8, rows - t * 8);
-        for (int x = tid; x < limit * D; x += kThreads) {
-          const int r = x / D, d = x % D;
+        for (int x = tid; x < limit * (D / 4); x += kThreads) {
+          const int r = x / (D / 4), d = x % (D / 4) * 4;
           const float m = fmaxf(fmaxf(sm.top[0][r], sm.top[1][r]), fmaxf(sm.top[2][r], sm.top[3][r]));
-          float acc = 0.f, l = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float l = 0.f;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const float f = exp2_mufu(sm.top[w][r] - m);
-            acc = fmaf(f, joined[w][r][d], acc);
+            add_scaled(acc, *reinterpret_cast<const float4*>(&joined[w][r][d]), f);
             l = fmaf(f, sm.sum[w][r], l);
           }
           const int row = t * 8 + r;
           if (parts == 1) {
-            T* out = reinterpret_cast<T*>(p.o) + (cur.r.q0 + row / group) * p.o_tok +
-                     (cur.head * group + row % group) * p.o_head;
-            out[d] = Half<T>::round(l == 0.f ? 0.f : acc / l);
+            store_row4<T>(place(row) + d, acc, l);
           } else {
-            float* at = mine_at + row * (D + 2);
-            __stcg(at + d, acc);
-            if (d == 0) {
-              __stcg(at + D, m);
-              __stcg(at + D + 1, l);
-            }
+            float* at = mine_at + row * D + d;
+            __stcg(reinterpret_cast<float4*>(at), acc);
+            if (d == 0) __stcg(reinterpret_cast<float2*>(mine_at + kRows * D) + row, make_float2(m, l));
           }
         }
         __syncthreads();
@@ -390,27 +484,33 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         int* counter = reinterpret_cast<int*>(p.work) + first;
         __threadfence();
         __syncthreads();
-        if (tid == 0) sm.last = atomicAdd(counter, 1) == parts - 1;
+        if (tid == 0) {
+          const int done = atomicAdd(counter, 1);
+          if (done == parts - 1) *counter = 0;  // as the next launch finds it
+          sm.last = done == parts - 1;
+        }
         __syncthreads();
         if (sm.last) {
           __threadfence();
-          for (int x = tid; x < rows * D; x += kThreads) {
-            const int row = x / D, d = x % D;
-            float m = kLowest, acc = 0.f, l = 0.f;
+          for (int x = tid; x < rows * (D / 4); x += kThreads) {
+            const int row = x / (D / 4), d = x % (D / 4) * 4;
+            float m = kLowest, l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            // (Four parts' loads are in flight at a time.)
+#pragma unroll 4
             for (int i = 0; i < parts; ++i) {
-              const float* at = slots + (i == 0 ? 2 * first + 1 : 2 * (first + i)) * slot_floats + row * (D + 2);
-              const float pm = __ldcg(at + D), pl = __ldcg(at + D + 1), po = __ldcg(at + d);
-              const float big = fmaxf(m, pm);
-              const float f = exp2_mufu(m - big), g = exp2_mufu(pm - big);
-              acc = acc * f + po * g;
-              l = l * f + pl * g;
+              const float* at = slots + (i == 0 ? 2 * first + 1 : 2 * (first + i)) * slot_floats;
+              const float2 st = __ldcg(reinterpret_cast<const float2*>(at + kRows * D) + row);
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(at + row * D + d));
+              const float big = fmaxf(m, st.x);
+              const float f = exp2_mufu(m - big), g = exp2_mufu(st.x - big);
+              acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+              add_scaled(acc, v, g);
+              l = fmaf(l, f, st.y * g);
               m = big;
             }
-            T* out = reinterpret_cast<T*>(p.o) + (cur.r.q0 + row / group) * p.o_tok +
-                     (cur.head * group + row % group) * p.o_head;
-            out[d] = Half<T>::round(l == 0.f ? 0.f : acc / l);
+            store_row4<T>(place(row) + d, acc, l);
           }
-          if (tid == 0) *counter = 0;  // as the next launch finds it
         }
       }
       fresh = true;
@@ -423,7 +523,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
 
 #define TB_TOKEN_ENTRY(name, T, D, NT)                                                                       \
   extern "C" __global__ void __launch_bounds__(kThreads, 2) name(const __grid_constant__ tb::AttnParams p) { \
-    static_assert(sizeof(Shared<D>) + 128 <= tb::token_smem_bytes(D), "shared memory reservation");          \
+    static_assert(sizeof(Shared<D, 8 * NT>) + 128 <= tb::token_smem_bytes(D, 8 * NT), "shared memory reservation");          \
     attention_tokens<T, D, NT>(p);                                                                           \
   }
 
