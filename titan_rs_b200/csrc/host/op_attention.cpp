@@ -90,7 +90,7 @@ tb_status launch_rows(Session* s, Stream* st, AttnCall* c) {
   uint64_t grid = ((uint64_t)c->p.tq * c->p.heads + 7) / 8;  // 8 rows (warps) per 256-thread CTA
   if (grid > (uint64_t)s->sm_count * 64) grid = (uint64_t)s->sm_count * 64;
   void* params[] = {&c->p};
-  return launch_builtin(s, st, fn, (unsigned)grid, 1, 1, 256, 0, params, entry);
+  return launch_overlapped(s, st, fn, (unsigned)grid, 1, 256, 0, params, entry);
 }
 
 // Whether 16-byte copies reach every row of Q, K and V.
@@ -177,8 +177,8 @@ tb_status launch_tiles(Session* s, Stream* st, AttnCall* c, uint64_t longest) {
   p.work = work;
   CUdeviceptr status = s->status.device;
   void* params[] = {&p, &mq, &mk, &mv, &status};
-  rc = launch_builtin(s, st, fn, (unsigned)grid, 1, 1, kTileThreads, (unsigned)tile_smem_bytes(p.dim), params,
-                      entry.c_str());
+  rc = launch_overlapped(s, st, fn, (unsigned)grid, 1, kTileThreads, (unsigned)tile_smem_bytes(p.dim), params,
+                         entry.c_str());
   return rc;
 }
 
@@ -194,7 +194,7 @@ tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
   if ((rc = stream_workspace(s, st, token_workspace_bytes(ctas, c->p.token_rows, c->p.dim), &work))) return rc;
   c->p.work = work;
   void* params[] = {&c->p};
-  return launch_builtin(s, st, fn, (unsigned)ctas, 1, 1, kTokenThreads, (unsigned)token_smem_bytes(c->p.dim, c->p.token_rows), params,
+  return launch_overlapped(s, st, fn, (unsigned)ctas, 1, kTokenThreads, (unsigned)token_smem_bytes(c->p.dim, c->p.token_rows), params,
                         entry.c_str());
 }
 

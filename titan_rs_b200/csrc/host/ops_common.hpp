@@ -164,6 +164,33 @@ inline tb_status launch_builtin(Session* s, Stream* st, CUfunction fn, unsigned 
   return TB_OK;
 }
 
+// Launches a built-in kernel that begins by waiting for the grids before it
+// (griddepcontrol.wait), so that its blocks may be set up while those still run.
+inline tb_status launch_overlapped(Session* s, Stream* st, CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
+                                   unsigned shared_bytes, void** params, const char* candidate) {
+  const DriverApi* d = driver();
+  if (shared_bytes > 48 * 1024)
+    TB_CU("cuFuncSetAttribute",
+          d->cuFuncSetAttribute(fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)shared_bytes));
+  CUlaunchConfig cfg{};
+  cfg.gridDimX = gx;
+  cfg.gridDimY = gy;
+  cfg.gridDimZ = 1;
+  cfg.blockDimX = bx;
+  cfg.blockDimY = cfg.blockDimZ = 1;
+  cfg.sharedMemBytes = shared_bytes;
+  cfg.hStream = st->raw;
+  CUlaunchAttribute attr{};
+  attr.id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+  attr.value.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TB_CU("cuLaunchKernelEx", d->cuLaunchKernelEx(&cfg, fn, params, nullptr));
+  note_launch(candidate);
+  (void)s;
+  return TB_OK;
+}
+
 // CTA pairs (clusters of two along x) of a built-in pair kernel that can be resident at
 // once. The driver is asked once per kernel and session (each built-in pair kernel is
 // always launched with the same block and shared-memory size).

@@ -86,6 +86,14 @@ TB_BOTH constexpr int tile_smem_bytes(int dim) {
 }
 // The index arithmetic is shared by the kernels and a host test of it.
 #ifdef __CUDACC__
+// These kernels are launched with programmatic stream serialization (launch_overlapped):
+// the next one's blocks are set up while the one before still runs. Every thread calls this
+// before its first access to global memory; it returns when the grids before have ended and
+// their writes are visible.
+__device__ __forceinline__ void begin_after_earlier_grids() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 #define TB_INDEX_FN __device__ __forceinline__
 TB_INDEX_FN int load_index(const int* p) { return __ldg(p); }
 #else

@@ -24,6 +24,7 @@ __device__ __forceinline__ void store_as(__half* p, float x) { *p = __float2half
 
 template <typename T>
 __device__ __forceinline__ void attention_rows(const AttnParams& p) {
+  begin_after_earlier_grids();
   const int lane = threadIdx.x & 31;
   const int* cu_q = reinterpret_cast<const int*>(p.cu_q);
   const long long units = (long long)p.tq * p.heads;

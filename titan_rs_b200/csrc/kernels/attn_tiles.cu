@@ -380,6 +380,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
+  begin_after_earlier_grids();
   // ---- a CTA's share of the call, in key tiles, and the works (parts of items) of each class ----
   if (threadIdx.x < kClasses) scratch->works[threadIdx.x] = 0;
   long long mine = 0;

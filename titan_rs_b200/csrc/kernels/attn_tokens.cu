@@ -172,6 +172,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = p.heads / p.kv_heads;
 
+  begin_after_earlier_grids();
   // ---- this CTA's run of tiles ----
   const auto units = [&](int b) { return tiles_of(p, request_of(p, b)); };
   const Stretch stretch = count_units<kThreads>(p.batch, sm.scan, units);
