@@ -437,10 +437,11 @@ tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, const tb_tenso
  * Writes block_table's new entries, seq_lens = context + new, cu_seqlens (the running sum of
  * new_lens, [batch + 1]), slot_map (a slot for each packed token, -1 past the last one) and
  * status = {pages taken from the front of free_pages, requests refused}.
- * A request is refused when a length is negative, its pages exceed the row, its tokens pass
- * the end of slot_map, or free_pages ends before its pages (later requests that need pages
+ * A request is refused when a length is negative or context + new passes 2^31 - 1, its pages
+ * exceed the row, its tokens pass the end of slot_map, or free_pages ends before its pages (later requests that need pages
  * are then refused too): its seq_lens is its context, its slots are -1, its row is not
- * written. Up to 16384 requests. Attribute page_size (required). */
+ * written. Up to 16384 requests. Attribute page_size (required). Outputs that share memory with
+ * an input or each other are refused. */
 tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const tb_tensor* context_lens,
                         const tb_tensor* new_lens, const tb_tensor* free_pages, const tb_tensor* block_table,
                         const tb_tensor* seq_lens, const tb_tensor* cu_seqlens, const tb_tensor* slot_map,

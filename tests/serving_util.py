@@ -109,7 +109,7 @@ def plan_reference(ctx, new, free, table, tokens, page):
         c, n = max(int(ctx[b]), 0), max(int(new[b]), 0)
         held, wanted = -(-c // page), -(-(c + n) // page)
         cu[b] = min(at, tokens)
-        fits = ctx[b] >= 0 and new[b] >= 0 and wanted <= width and at + n <= tokens
+        fits = ctx[b] >= 0 and new[b] >= 0 and c + n < 2 ** 31 and wanted <= width and at + n <= tokens
         need = wanted - held if fits else 0
         if fits and taken + need <= len(free):
             table[b, held:wanted] = free[taken:taken + need]

@@ -89,6 +89,20 @@ def test_plan_refuses_requests_and_says_how_many(session, rt):
     assert_plan(session, rt, [0, 0, 0], [10, 10, 10], [1, 2, 3, 4], np.zeros((3, 2), np.int32), 15, page)
     assert_plan(session, rt, [3, 3], [2, 2], [7], np.array([[2 ** 31 - 1], [-4]], np.int32), 4, page)
     assert_plan(session, rt, [2 ** 31 - 1], [2 ** 31 - 1], [7], np.array([[1, 1]], np.int32), 4, 2 ** 31 - 1)
+    assert_plan(session, rt, [2 ** 31 - 2, 2 ** 31 - 3], [3, 2], [7, 8], np.array([[1, 1], [0, 5]], np.int32), 9,
+                2 ** 31 - 1)
+
+
+def test_plan_refuses_outputs_that_share_memory(session, rt):
+    ctx, new, free = (ints(session, rt, x) for x in ([5, 6], [1, 1], [7, 8, 9]))
+    outs = [ints(session, rt, np.full((2, 3), -1)), ints(session, rt, [0, 0]), ints(session, rt, [0, 0, 0]),
+            ints(session, rt, [0, 0]), ints(session, rt, [0, 0])]
+    for i, other in ((1, ctx), (3, new), (3, outs[4]), (4, outs[1])):
+        bad = list(outs)
+        bad[i] = other
+        with pytest.raises(tb.ExecutionError, match="share no memory"):
+            rt.execute(tb.OpRequest("kv_cache.plan", [ctx, new, free], [spec_of(x) for x in outs], {"page_size": 16}),
+                       output=bad)
 
 
 def test_plan_strided_table(session, rt):

@@ -1,6 +1,8 @@
 // "kv_cache.plan" and "kv_cache.append": the bookkeeping and the write of a paged key/value
 // cache, beside the attention that reads it (op_attention.cpp). No counterpart in the
 // reference; the checks and messages follow the manner of its operators.
+#include <algorithm>
+
 #include "../kernels/kv_params.cuh"
 #include "ops_common.hpp"
 
@@ -8,7 +10,7 @@ using namespace tb;
 
 namespace {
 
-// Requests the plan kernel takes in one call (its shared memory holds a word for each).
+// Requests the plan kernel takes in one call (its shared memory holds two words for each).
 constexpr uint64_t kMaxPlanRequests = 16384;
 
 bool same_rows(const tb_tensor* rows, const tb_tensor* cache) {
@@ -85,10 +87,13 @@ extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, con
   p.chunks = (int)(D * size / chunk);
   CUfunction fn = nullptr;
   if ((rc = builtin_function(s, "kv_cache", entry, &fn))) return rc;
-  uint64_t grid = (T * H * (uint64_t)p.chunks + 255) / 256;
-  if (grid > (uint64_t)s->sm_count * 16) grid = (uint64_t)s->sm_count * 16;
+  // A pass of a block covers kAppendThreads chunks of whole tokens. Few passes get a block each;
+  // many are taken four to a thread, as the kernel unrolls.
+  const uint64_t at_once = std::max<uint64_t>(1, kAppendThreads / (2 * H * (uint64_t)p.chunks));
+  const uint64_t passes = (T + at_once - 1) / at_once, few = 2 * (uint64_t)s->sm_count;
+  const uint64_t grid = passes <= few ? passes : std::max(few, (passes + 3) / 4);
   void* params[] = {&p};
-  if ((rc = launch_builtin(s, st, fn, (unsigned)grid, 2, 1, 256, 0, params, entry))) return rc;
+  if ((rc = launch_overlapped(s, st, fn, (unsigned)grid, 1, kAppendThreads, 0, params, entry))) return rc;
   return record_event(s, st, nullptr, out);
 }
 
@@ -133,12 +138,43 @@ extern "C" tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const
       (rc = strided_buffer(s, slot_map, "kv_cache.plan slot_map", &bm)) ||
       (rc = strided_buffer(s, status, "kv_cache.plan status", &bs)) || (rc = activate(s)))
     return rc;
+  // The kernel's blocks read the inputs while others write.
+  const struct {
+    uint64_t ptr, bytes;
+  } ranges[] = {{bt->ptr, 4 * ((B - 1) * (uint64_t)step_of(block_table, 0) + W)},
+                {bl->ptr, 4 * B},
+                {bcu->ptr, 4 * (B + 1)},
+                {bm->ptr, 4 * T},
+                {bs->ptr, 8},
+                {bc->ptr, 4 * B},
+                {bn->ptr, 4 * B},
+                {bf->ptr, 4 * F}};
+  for (int i = 0; i < 5; ++i)
+    for (int j = i + 1; j < 8; ++j)
+      if (ranges[i].ptr < ranges[j].ptr + ranges[j].bytes && ranges[j].ptr < ranges[i].ptr + ranges[i].bytes)
+        return contract("kv_cache.plan requires outputs that share no memory with the inputs or each other");
   CUfunction fn = nullptr;
   if ((rc = builtin_function(s, "kv_cache", "kv_plan", &fn))) return rc;
-  int batch = (int)B, n_free = (int)F, width = (int)W, tokens = (int)T, pg = (int)page;
-  long long row = step_of(block_table, 0);
-  void* params[] = {&bc->ptr, &bn->ptr, &bf->ptr, &bt->ptr, &bl->ptr,  &bcu->ptr, &bm->ptr,
-                    &bs->ptr, &batch,   &n_free,  &width,   &row,      &tokens,   &pg};
-  if ((rc = launch_builtin(s, st, fn, 1, 1, 1, 1024, (unsigned)(B * sizeof(int)), params, "kv_plan"))) return rc;
+  PlanParams p{};
+  p.ctx = bc->ptr;
+  p.add = bn->ptr;
+  p.free_pages = bf->ptr;
+  p.table = bt->ptr;
+  p.lens = bl->ptr;
+  p.cu = bcu->ptr;
+  p.slots = bm->ptr;
+  p.status = bs->ptr;
+  p.table_row = step_of(block_table, 0);
+  p.batch = (int)B;
+  p.n_free = (int)F;
+  p.width = (int)W;
+  p.tokens = (int)T;
+  p.page = (int)page;
+  // A token a thread; more blocks than resident ones would only repeat the sums.
+  const uint64_t grid = std::min((std::max(T, 8 * B) + kPlanThreads - 1) / kPlanThreads, (uint64_t)s->sm_count * 2);
+  void* params[] = {&p};
+  if ((rc = launch_overlapped(s, st, fn, (unsigned)grid, 1, kPlanThreads, (unsigned)((2 * B + 1) * sizeof(int)), params,
+                              "kv_plan")))
+    return rc;
   return record_event(s, st, nullptr, out);
 }

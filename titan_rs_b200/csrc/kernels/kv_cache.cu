@@ -1,107 +1,181 @@
 // The paged key/value cache: the pages and slots of a step, and the write of its new rows.
+#include "attn_params.cuh"
 #include "kv_params.cuh"
 
 namespace {
 
 using namespace tb;
 
-// One row chunk of B bytes, cache[slot] = rows[token], for K (z = 0) and V (z = 1).
+// cache[slots[t]] = rows[t] for K and V, in chunks of 2, 4 or 16 bytes.
+//
+// A copy, bound by the HBM: every row is read and written once. A thread keeps its place in a
+// token's row (K or V, head, chunk) and steps over tokens, four at a time, so that the
+// divisions are done once and four loads are in flight.
 template <typename Chunk>
-__device__ __forceinline__ void append_rows(const char* __restrict__ rows, char* __restrict__ cache,
-                                            const int* __restrict__ slots, int tokens, int heads, int chunks, int page,
-                                            long long limit, long long r_tok, long long r_head, long long c_page,
-                                            long long c_tok, long long c_head) {
-  const long long per_token = (long long)heads * chunks, total = tokens * per_token;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(i / per_token), rest = (int)(i % per_token);
-    const int h = rest / chunks, c = rest % chunks;
-    const int slot = __ldg(slots + t);
-    if (slot < 0 || slot >= limit) continue;
-    const Chunk x = *reinterpret_cast<const Chunk*>(rows + t * r_tok + h * r_head + c * (long long)sizeof(Chunk));
-    *reinterpret_cast<Chunk*>(cache + (slot / page) * c_page + (slot % page) * c_tok + h * c_head +
-                              c * (long long)sizeof(Chunk)) = x;
+__device__ __forceinline__ void append_rows(const AppendParams& p) {
+  begin_after_earlier_grids();
+  const int per = p.heads * p.chunks, places = 2 * per;  // a token's chunks of K, and of both
+  const int at_once = max(1, kAppendThreads / places);   // tokens of a pass of the block
+  const int local = places <= kAppendThreads ? threadIdx.x / places : 0;
+  if (local >= at_once) return;
+  const long long step = (long long)gridDim.x * at_once;
+  const int* const slots = reinterpret_cast<const int*>(p.slots);
+  for (int place = places <= kAppendThreads ? threadIdx.x % places : threadIdx.x; place < places;
+       place += kAppendThreads) {
+    const bool v = place >= per;
+    const int h = (v ? place - per : place) / p.chunks, c = (v ? place - per : place) % p.chunks;
+    const char* const from =
+        reinterpret_cast<const char*>(v ? p.v : p.k) + h * (v ? p.v_head : p.k_head) + c * (int)sizeof(Chunk);
+    char* const to = reinterpret_cast<char*>(v ? p.v_cache : p.k_cache) + h * (v ? p.vc_head : p.kc_head) +
+                     c * (int)sizeof(Chunk);
+    const long long r_tok = v ? p.v_tok : p.k_tok, c_page = v ? p.vc_page : p.kc_page, c_tok = v ? p.vc_tok : p.kc_tok;
+    for (long long t = (long long)blockIdx.x * at_once + local; t < p.tokens; t += 4 * step) {
+      Chunk x[4];
+      int slot[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = t + i * step < p.tokens;
+        slot[i] = in ? __ldg(slots + t + i * step) : -1;
+        if (in) x[i] = *reinterpret_cast<const Chunk*>(from + (t + i * step) * r_tok);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (slot[i] >= 0 && slot[i] < p.limit)
+          *reinterpret_cast<Chunk*>(to + (slot[i] / p.page) * c_page + (slot[i] % p.page) * c_tok) = x[i];
+    }
   }
 }
 
-template <typename Chunk>
-__device__ __forceinline__ void append_body(const AppendParams& p) {
-  const bool v = blockIdx.y != 0;
-  append_rows<Chunk>(reinterpret_cast<const char*>(v ? p.v : p.k), reinterpret_cast<char*>(v ? p.v_cache : p.k_cache),
-                     reinterpret_cast<const int*>(p.slots), p.tokens, p.heads, p.chunks, p.page, p.limit,
-                     v ? p.v_tok : p.k_tok, v ? p.v_head : p.k_head, v ? p.vc_page : p.kc_page,
-                     v ? p.vc_tok : p.kc_tok, v ? p.vc_head : p.kc_head);
+// The sum of `mine` over the threads before this one, and over all (total). `words` holds one
+// word a warp and is free again when the next barrier has passed.
+template <int kThreads>
+__device__ __forceinline__ long long sum_before(long long mine, long long* words, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += x;
+  }
+  if (lane == 31) words[warp] = upto;
+  __syncthreads();
+  long long before = upto - mine;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += words[w];
+    total += words[w];
+  }
+  return before;
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256) kv_append_16(const __grid_constant__ tb::AppendParams p) {
-  append_body<uint4>(p);
+extern "C" __global__ void __launch_bounds__(tb::kAppendThreads)
+    kv_append_16(const __grid_constant__ tb::AppendParams p) {
+  append_rows<uint4>(p);
 }
-extern "C" __global__ void __launch_bounds__(256) kv_append_4(const __grid_constant__ tb::AppendParams p) {
-  append_body<uint32_t>(p);
+extern "C" __global__ void __launch_bounds__(tb::kAppendThreads) kv_append_4(const __grid_constant__ tb::AppendParams p) {
+  append_rows<uint32_t>(p);
 }
-extern "C" __global__ void __launch_bounds__(256) kv_append_2(const __grid_constant__ tb::AppendParams p) {
-  append_body<uint16_t>(p);
+extern "C" __global__ void __launch_bounds__(tb::kAppendThreads) kv_append_2(const __grid_constant__ tb::AppendParams p) {
+  append_rows<uint16_t>(p);
 }
 
-// Pages and slots of one step, one CTA. For request b with ctx tokens cached and `add` new ones:
+// Pages and slots of one step. For request b with ctx tokens cached and `add` new ones:
 //   held = ceil(ctx / page), wanted = ceil((ctx + add) / page), need = wanted - held;
 //   its new pages are free[first .. first + need), first = the sum of need over earlier requests;
 //   a new token at position x has slot page_of(x / page) * page + x % page.
 // A request is refused, keeping ctx tokens and giving its new tokens slot -1, when a length
-// is negative, its row of the table is too short, its tokens pass the slot map's end, or the
-// free list ends before its pages. One thread walks the requests (the sums), then all
-// threads fill in the tokens.
-extern "C" __global__ void __launch_bounds__(1024)
-    kv_plan(const int* __restrict__ ctx, const int* __restrict__ add, const int* __restrict__ free_pages,
-            int* __restrict__ table, int* __restrict__ lens, int* __restrict__ cu, int* __restrict__ slots,
-            int* __restrict__ status, int batch, int n_free, int width, long long table_row, int tokens, int page) {
-  extern __shared__ int first_of[];  // first new page of each request, or -1 when refused
-  if (threadIdx.x == 0) {
-    long long at = 0, taken = 0, given = 0;
-    int refused = 0;
-    for (int b = 0; b < batch; ++b) {
-      const long long c = max(ctx[b], 0), n = max(add[b], 0);
-      const long long held = (c + page - 1) / page, wanted = (c + n + page - 1) / page;
-      cu[b] = (int)(at < tokens ? at : tokens);
-      const bool fits = ctx[b] >= 0 && add[b] >= 0 && wanted <= width && at + n <= tokens;
-      const long long need = fits ? wanted - held : 0;
-      const bool served = fits && taken + need <= n_free;
-      first_of[b] = served ? (int)taken : -1;
-      lens[b] = (int)(served ? c + n : c);
-      if (served) given += need;
-      refused += served ? 0 : 1;
-      taken += need;
-      at += n;
-    }
-    cu[batch] = (int)(at < tokens ? at : tokens);
-    status[0] = (int)given;
-    status[1] = refused;
+// is negative or passes 2^31 - 1, its row of the table is too short, its tokens pass the slot
+// map's end, or the free list ends before its pages.
+//
+// Some kilobytes, so a few memory latencies and the launch are all there is: every block
+// repeats the sums over the requests (two scans, of tokens and of pages) instead of waiting for
+// another's, keeps each request's first token and first page in shared memory, and fills in its
+// share of the tokens, requests and table rows. Old pages are only read and new ones only
+// taken from the free list, so no block needs what another writes.
+extern "C" __global__ void __launch_bounds__(tb::kPlanThreads) kv_plan(const __grid_constant__ tb::PlanParams p) {
+  extern __shared__ int words[];
+  int* const start = words;                 // first token of request b (batch + 1 of them)
+  int* const first = words + p.batch + 1;   // its first new page's place in the free list, or -1 when refused
+  __shared__ long long sums[2][kPlanThreads / 32];
+  __shared__ int given, refused;
+  const int* const ctx = reinterpret_cast<const int*>(p.ctx);
+  const int* const add = reinterpret_cast<const int*>(p.add);
+  const int* const free_pages = reinterpret_cast<const int*>(p.free_pages);
+  int* const table = reinterpret_cast<int*>(p.table);
+  if (threadIdx.x == 0) given = refused = 0;
+  begin_after_earlier_grids();
+
+  const int per = (p.batch + kPlanThreads - 1) / kPlanThreads;
+  const int lo = min((int)threadIdx.x * per, p.batch), hi = min(lo + per, p.batch);
+  const auto pages = [&](long long tokens) { return (tokens + p.page - 1) / p.page; };
+  long long tokens = 0, total = 0;
+  for (int b = lo; b < hi; ++b) tokens += max(__ldg(add + b), 0);
+  long long at = sum_before<kPlanThreads>(tokens, sums[0], total);
+  long long need = 0;
+  for (int b = lo; b < hi; ++b) {
+    const long long c = __ldg(ctx + b), n = __ldg(add + b);
+    const bool fits = c >= 0 && n >= 0 && c + n <= 0x7fffffff && pages(c + n) <= p.width && at + n <= p.tokens;
+    const int own = fits ? (int)(pages(c + n) - pages(c)) : -1;
+    start[b] = (int)min(at, (long long)p.tokens);
+    first[b] = own;
+    need += max(own, 0);
+    at += max(n, 0ll);
+  }
+  if (threadIdx.x == 0) start[p.batch] = (int)min(total, (long long)p.tokens);
+  long long taken = sum_before<kPlanThreads>(need, sums[1], total);
+  int my_given = 0, my_refused = 0;
+  for (int b = lo; b < hi; ++b) {
+    const int own = first[b];
+    const bool served = own >= 0 && taken + own <= p.n_free;
+    first[b] = served ? (int)taken : -1;
+    taken += max(own, 0);
+    my_given += served ? own : 0;
+    my_refused += served ? 0 : 1;
+  }
+  if (blockIdx.x == 0 && (my_given || my_refused)) {
+    atomicAdd(&given, my_given);
+    atomicAdd(&refused, my_refused);
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < batch; b += blockDim.x) {
-    if (first_of[b] < 0) continue;
-    const int held = (int)(((long long)ctx[b] + page - 1) / page);
-    const int wanted = (int)(((long long)ctx[b] + add[b] + page - 1) / page);
-    for (int i = held; i < wanted; ++i) table[b * table_row + i] = free_pages[first_of[b] + i - held];
+
+  const int tid = blockIdx.x * kPlanThreads + threadIdx.x, threads = gridDim.x * kPlanThreads;
+  if (tid == 0) {
+    reinterpret_cast<int*>(p.status)[0] = given;
+    reinterpret_cast<int*>(p.status)[1] = refused;
   }
-  __syncthreads();
-  for (int t = threadIdx.x; t < tokens; t += blockDim.x) {
-    int lo = 0, hi = batch + 1;  // the last request that starts at or before token t
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (cu[mid] <= t) lo = mid + 1;
-      else hi = mid;
+  for (int b = tid; b <= p.batch; b += threads) {
+    reinterpret_cast<int*>(p.cu)[b] = start[b];
+    if (b < p.batch) {
+      const int c = max(__ldg(ctx + b), 0);
+      reinterpret_cast<int*>(p.lens)[b] = first[b] >= 0 ? c + __ldg(add + b) : c;
     }
-    const int b = lo - 1;
+  }
+  // The new entries of the table, a warp a request.
+  for (int b = tid >> 5; b < p.batch; b += threads >> 5) {
+    if (first[b] < 0) continue;
+    const long long c = __ldg(ctx + b);
+    const int held = (int)pages(c), wanted = (int)pages(c + __ldg(add + b));
+    for (int i = held + (int)(threadIdx.x & 31); i < wanted; i += 32)
+      table[b * p.table_row + i] = __ldg(free_pages + first[b] + i - held);
+  }
+  for (int t = tid; t < p.tokens; t += threads) {
+    int below = 0, above = p.batch + 1;  // the last request that starts at or before token t
+    while (below < above) {
+      const int mid = (below + above) >> 1;
+      if (start[mid] <= t) below = mid + 1;
+      else above = mid;
+    }
+    const int b = below - 1;
     int slot = -1;
-    if (b < batch && first_of[b] >= 0) {
-      const int x = ctx[b] + t - cu[b];
-      const int id = table[b * table_row + x / page];
-      const long long at = (long long)id * page + x % page;
-      if (id >= 0 && at <= 0x7fffffff) slot = (int)at;
+    if (b < p.batch && first[b] >= 0) {
+      const int c = __ldg(ctx + b), x = c + t - start[b], index = x / p.page, held = (int)pages(c);
+      const int id = index < held ? table[b * p.table_row + index] : __ldg(free_pages + first[b] + index - held);
+      const long long place = (long long)id * p.page + x % p.page;
+      if (id >= 0 && place <= 0x7fffffff) slot = (int)place;
     }
-    slots[t] = slot;
+    reinterpret_cast<int*>(p.slots)[t] = slot;
   }
 }
