@@ -47,7 +47,7 @@ constexpr uint32_t kFailMma = 0x56020000u;
 constexpr uint32_t kFailSoftmax = 0x56030000u;
 constexpr uint32_t kFailClear = 0x56040000u;
 constexpr uint32_t kFailSchedule = 0x56050000u;
-constexpr uint32_t kControlRegs = 72, kSoftmaxRegs = 216;
+constexpr uint32_t kControlRegs = 88, kSoftmaxRegs = 208;
 static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kTileThreads * kTileLaunchRegs,
               "the warpgroups' registers exceed the launch allocation");
 
@@ -894,7 +894,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
 
 }  // namespace
 
-// One CTA per SM at 168 registers a thread; the warpgroups re-divide them (56 and 216).
+// One CTA per SM at 168 registers a thread; the warpgroups re-divide them (88 and 208).
 #define TB_TILE_ENTRY(suffix, T, HD)                                                                                \
   extern "C" __global__ void __launch_bounds__(tb::kTileThreads, 1)                                                 \
       attention_tiles_##suffix(const __grid_constant__ tb::AttnParams p, const __grid_constant__ CUtensorMap tmap_q, \
