@@ -71,6 +71,7 @@ typedef struct tb_event tb_event;
 typedef struct tb_kernel tb_kernel;
 typedef struct tb_comm tb_comm;
 typedef struct tb_graph_exec tb_graph_exec;
+typedef struct tb_request tb_request;
 
 /* DeviceFingerprint (titan-types/src/lib.rs:28-38); capability_revision is
  * "sm_<major><minor>" as in CudaDiscovery (titan-backend-cuda/src/lib.rs:221-226). */
@@ -296,6 +297,18 @@ tb_status tb_execute(tb_session* session, tb_stream* stream, const char* op, con
 tb_status tb_execute_outputs(tb_session* session, tb_stream* stream, const char* op, const tb_tensor* inputs,
                              uint32_t num_inputs, const tb_tensor* outputs, uint32_t num_outputs,
                              const tb_attr* attrs, uint32_t num_attrs, tb_event** out);
+
+/* No counterpart in the reference. A request kept for repeated launches over the same
+ * tensors (a serving step): tb_request_create copies the arguments of tb_execute_outputs and
+ * holds the session, the stream and the tensors' buffers until tb_request_release;
+ * tb_request_enqueue runs it like tb_execute_outputs (the operator's checks included; `out`
+ * may be NULL for no event). A request may be enqueued from several threads, and released
+ * once, when none uses it. */
+tb_status tb_request_create(tb_session* session, tb_stream* stream, const char* op, const tb_tensor* inputs,
+                            uint32_t num_inputs, const tb_tensor* outputs, uint32_t num_outputs,
+                            const tb_attr* attrs, uint32_t num_attrs, tb_request** out);
+tb_status tb_request_enqueue(const tb_request* request, tb_event** out);
+void tb_request_release(tb_request* request);
 
 /* Runtime::compile (titan-runtime/src/lib.rs:3472-3483) over the Graph IR
  * (titan-graph/src/graph.rs:72-105), shaped like the core pipeline

@@ -296,5 +296,44 @@ def test_bound_requests_hold_their_buffers(session):
     b.enqueue()
     np.testing.assert_allclose(y.to_numpy(rt.stream), want, rtol=1e-5)
     rt.stream.release()
-    with pytest.raises(tb.ExecutionError, match="released"):
-        b.enqueue()
+    b.enqueue()  # and their stream
+    other = tb.Session(0)
+    foreign = upload(other, other.create_stream(), np.ones((4, 64), np.float32))
+    foreign.session = session
+    with pytest.raises(tb.ExecutionError, match="foreign buffer"):
+        tb.Runtime(session).bind(tb.OpRequest("softmax", [foreign], [tb.TensorSpec(DType.F32, (4, 64))]), y)
+    with pytest.raises(tb.ExecutionError, match="same shape"):  # an operator's checks run at every enqueue
+        tb.Runtime(session).bind(tb.OpRequest("softmax", [y], [tb.TensorSpec(DType.F32, (2, 64))]), y).enqueue()
+
+
+def test_bound_requests_from_two_threads(session):
+    """Two host threads on one stream, with an operator that takes the stream's workspace."""
+    import threading
+    rt = tb.Runtime(session)
+    batch, h, hk, d, page = 3, 8, 2, 128, 16
+    lens = [3000, 70, 1100]
+    need = [-(-n // page) for n in lens]
+    table = np.full((batch, max(need)), -1, np.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = np.arange(at, at + n)
+        at += n
+    cache = [upload(session, rt.stream, rows((at, page, hk, d), DType.BF16, 900 + i), DType.BF16) for i in range(2)]
+    ins = cache + [ints(session, rt, table), ints(session, rt, lens)]
+    bound = []
+    for tokens in (1, 20):  # the token kernel and the tile kernel, whose workspaces differ in size
+        q = upload(session, rt.stream, rows((batch * tokens, h, d), DType.BF16, 910), DType.BF16)
+        cu = ints(session, rt, np.arange(batch + 1) * tokens)
+        request = tb.OpRequest("attention.paged", [q, *ins, cu], [spec_of(q)], {"max_query_len": tokens})
+        bound.append(rt.bind(request, tb.TensorHandle.allocate(session, DType.BF16, q.shape)))
+        bound[-1].enqueue()
+    session.synchronize(rt.stream)
+    want = [b.outputs[0].to_numpy(rt.stream) for b in bound]
+    threads = [threading.Thread(target=lambda b=b: [b.enqueue() for _ in range(200)]) for b in bound]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    session.synchronize(rt.stream)
+    for b, w in zip(bound, want):
+        np.testing.assert_array_equal(b.outputs[0].to_numpy(rt.stream), w)

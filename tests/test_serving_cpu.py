@@ -179,6 +179,18 @@ def test_python_requests_name_their_outputs():
         rt.bind(tb.OpRequest("kv_cache.append", [handle] * 2, [spec, spec]))
 
 
+def test_request_creation_checks_its_arguments():
+    L, t, handle = N.lib(), tensor(BF, (2, 2, 2)), ctypes.c_void_p(0)
+    ins = (N.Tensor * 1)(t)
+    for op, place, keyword in ((None, ctypes.byref(handle), "operator name"), (b"softmax", None, "handle"),
+                               (b"softmax", ctypes.byref(handle), "null session")):
+        assert L.tb_request_create(None, None, op, ins, 1, ins, 1, None, 0, place) == N.TB_ERR_INVALID
+        assert keyword in N.last_error()[1]
+    assert L.tb_request_create(None, None, b"softmax", None, 1, ins, 1, None, 0, ctypes.byref(handle)) == N.TB_ERR_INVALID
+    assert L.tb_request_enqueue(None, None) == N.TB_ERR_INVALID and N.last_error()[1] == "null request"
+    L.tb_request_release(None)
+
+
 HARNESS = r"""
 #include <cstdio>
 #include "attn_params.cuh"

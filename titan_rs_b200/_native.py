@@ -152,6 +152,10 @@ _SIGNATURES = {
                         ctypes.POINTER(Attr), _U32, _PP]),
     "tb_execute_outputs": (_S, [_P, _P, ctypes.c_char_p, ctypes.POINTER(Tensor), _U32, ctypes.POINTER(Tensor), _U32,
                                 ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_request_create": (_S, [_P, _P, ctypes.c_char_p, ctypes.POINTER(Tensor), _U32, ctypes.POINTER(Tensor), _U32,
+                               ctypes.POINTER(Attr), _U32, _PP]),
+    "tb_request_enqueue": (_S, [_P, _PP]),
+    "tb_request_release": (None, [_P]),
     "tb_op_attention_varlen": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 6 + [ctypes.POINTER(Attr), _U32, _PP]),
     "tb_op_attention_paged": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 7 + [ctypes.POINTER(Attr), _U32, _PP]),
     "tb_op_kv_append": (_S, [_P, _P] + [ctypes.POINTER(Tensor)] * 5 + [ctypes.POINTER(Attr), _U32, _PP]),

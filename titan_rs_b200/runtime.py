@@ -344,34 +344,37 @@ class Runtime:
 
 
 class BoundRequest:
-    """A request over fixed tensors (Runtime.bind): enqueue() launches it on the runtime's stream
-    with one native call and no event. It holds the tensors' buffers until it is dropped."""
+    """A request over fixed tensors (Runtime.bind, tb_request_*): enqueue() launches it on the
+    runtime's stream with one native call and no event. It holds its session, stream and
+    buffers until it is dropped."""
 
     def __init__(self, runtime: Runtime, request: OpRequest, outputs: list):
         self.runtime = runtime
         self.outputs = runtime._result(request, outputs)
         self._name = request.operator
-        self._args, self._keep = runtime._arguments(request.operator, request, outputs, dict(request.attrs))
-        self._session, self._stream = runtime.session, runtime.stream
-        self._call = N.lib().tb_execute_outputs
-        self._buffers = [t.buffer for t in [*request.inputs, *outputs]]
-        self._held = [b.ptr for b in self._buffers]
-        for ptr in self._held:
-            N.lib().tb_buffer_retain(ptr)
+        self._ptr = None
+        self._lib = N.lib()
+        args, _keep = runtime._arguments(request.operator, request, outputs, dict(request.attrs))
+        handle = ctypes.c_void_p(0)
+        self._check(self._lib.tb_request_create(*args, ctypes.byref(handle)))
+        self._ptr = handle
+        self._enqueue = self._lib.tb_request_enqueue
+
+    def _check(self, status: int) -> None:
+        if status != N.TB_OK:
+            op, detail = N.last_error()
+            raise ExecutionError(self._name, op or "launch", detail, status)
 
     def enqueue(self) -> None:
-        if self._session.ptr != self._args[0] or self._stream.ptr != self._args[1]:
-            raise ExecutionError(self._name, "contract", "the request's session or stream was released")
-        st = self._call(*self._args, None)
-        if st != N.TB_OK:
-            op, detail = N.last_error()
-            raise ExecutionError(self._name, op or "launch", detail, st)
+        status = self._enqueue(self._ptr, None)
+        if status != N.TB_OK:
+            self._check(status)
 
     def __del__(self):
-        held, self._held = getattr(self, "_held", []), []
+        ptr, self._ptr = getattr(self, "_ptr", None), None
         try:
-            for ptr in held:
-                N.lib().tb_buffer_release(ptr)
+            if ptr:
+                self._lib.tb_request_release(ptr)
         except Exception:
             pass
 
