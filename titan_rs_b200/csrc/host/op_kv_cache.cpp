@@ -153,8 +153,11 @@ extern "C" tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const
     for (int j = i + 1; j < 8; ++j)
       if (ranges[i].ptr < ranges[j].ptr + ranges[j].bytes && ranges[j].ptr < ranges[i].ptr + ranges[i].bytes)
         return contract("kv_cache.plan requires outputs that share no memory with the inputs or each other");
+  // Large batches want more threads for the sums, small ones fewer to wait for.
+  const unsigned threads = B > 256 ? 512 : 256;
+  const char* entry = B > 256 ? "kv_plan_512" : "kv_plan_256";
   CUfunction fn = nullptr;
-  if ((rc = builtin_function(s, "kv_cache", "kv_plan", &fn))) return rc;
+  if ((rc = builtin_function(s, "kv_cache", entry, &fn))) return rc;
   PlanParams p{};
   p.ctx = bc->ptr;
   p.add = bn->ptr;
@@ -171,10 +174,10 @@ extern "C" tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const
   p.tokens = (int)T;
   p.page = (int)page;
   // A token a thread; more blocks than resident ones would only repeat the sums.
-  const uint64_t grid = std::min((std::max(T, 8 * B) + kPlanThreads - 1) / kPlanThreads, (uint64_t)s->sm_count * 2);
+  const uint64_t grid = std::min((std::max(T, 8 * B) + threads - 1) / threads, (uint64_t)s->sm_count * 2);
   void* params[] = {&p};
-  if ((rc = launch_overlapped(s, st, fn, (unsigned)grid, 1, kPlanThreads, (unsigned)((2 * B + 1) * sizeof(int)), params,
-                              "kv_plan")))
+  if ((rc = launch_overlapped(s, st, fn, (unsigned)grid, 1, threads, (unsigned)((2 * B + 1) * sizeof(int)), params,
+                              entry)))
     return rc;
   return record_event(s, st, nullptr, out);
 }

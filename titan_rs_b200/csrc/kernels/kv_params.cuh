@@ -5,7 +5,7 @@
 
 namespace tb {
 
-constexpr int kAppendThreads = 256, kPlanThreads = 256;
+constexpr int kAppendThreads = 256;
 
 struct AppendParams {
   uint64_t k, v, k_cache, v_cache, slots;
