@@ -337,3 +337,63 @@ def test_bound_requests_from_two_threads(session):
     session.synchronize(rt.stream)
     for b, w in zip(bound, want):
         np.testing.assert_array_equal(b.outputs[0].to_numpy(rt.stream), w)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_graphs_of_one_stream_replay_side_by_side(session, tokens):
+    """Two graphs captured on one stream, and eager calls, keep their partial results apart: replayed at
+    the same time on three streams, each gives its own inputs' result every time."""
+    rt = tb.Runtime(session)
+    batch, h, hk, d, page, n = 2, 8, 2, 128, 16, 5000
+    pages = -(-n // page)
+    table = ints(session, rt, np.arange(batch * pages).reshape(batch, pages))
+    lens, cu = ints(session, rt, [n, n - 700]), ints(session, rt, np.arange(batch + 1) * tokens)
+    graphs, outs, want, bound = [], [], [], []
+    for g in range(3):
+        cache = [upload(session, rt.stream, rows((batch * pages, page, hk, d), DType.F16, 950 + 3 * g + i), DType.F16)
+                 for i in range(2)]
+        q = upload(session, rt.stream, rows((batch * tokens, h, d), DType.F16, 960 + g), DType.F16)
+        out = tb.TensorHandle.allocate(session, DType.F16, q.shape)
+        request = tb.OpRequest("attention.paged", [q, *cache, table, lens, cu], [spec_of(out)],
+                               {"max_query_len": tokens})
+        bound.append(rt.bind(request, out))
+        bound[-1].enqueue()
+        want.append(out.to_numpy(rt.stream))
+        outs.append(out)
+        if g < 2:
+            session.capture_begin(rt.stream)
+            bound[-1].enqueue()
+            graphs.append(session.capture_end(rt.stream))
+    session.synchronize(rt.stream)
+    zero = np.zeros(outs[0].shape, np.float16)
+    for t in outs:
+        session.wait(session.upload(rt.stream, t.buffer, zero))
+    streams = [session.create_stream() for _ in range(2)]
+    for _ in range(100):
+        graphs[0].launch(streams[0])
+        graphs[1].launch(streams[1])
+        bound[2].enqueue()
+    for st in (*streams, rt.stream):
+        session.synchronize(st)
+    for t, w in zip(outs, want):
+        np.testing.assert_array_equal(t.to_numpy(rt.stream), w)
+    for g in graphs:
+        g.release()
+
+
+def test_an_invalid_capture_leaves_the_stream_usable(session):
+    rt = tb.Runtime(session)
+    x = upload(session, rt.stream, rows((40, 4, 64), DType.BF16, 1), DType.BF16)
+    cu = ints(session, rt, [0, 40])
+    b = rt.bind(tb.OpRequest("attention.varlen", [x, x, x, cu], [spec_of(x)], {}),
+                tb.TensorHandle.allocate(session, DType.BF16, x.shape))
+    b.enqueue()
+    want = b.outputs[0].to_numpy(rt.stream)
+    session.capture_begin(rt.stream)
+    b.enqueue()
+    with pytest.raises(tb.HalError):  # a host wait on a capturing stream invalidates the capture
+        session.synchronize(rt.stream)
+    with pytest.raises(tb.HalError):
+        session.capture_end(rt.stream)
+    b.enqueue()
+    np.testing.assert_array_equal(b.outputs[0].to_numpy(rt.stream), want)

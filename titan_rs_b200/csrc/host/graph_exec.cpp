@@ -21,6 +21,7 @@ struct GraphExec : RefCounted {
   Session* session = nullptr;
   CUgraphExec exec = nullptr;
   std::vector<CUdeviceptr> work;  // workspace of its operators (stream_workspace)
+  std::atomic<uint64_t> work_epoch{0};
 };
 
 }  // namespace tb
@@ -38,6 +39,7 @@ tb_status tb_capture_begin(tb_session* session, tb_stream* stream) {
   rc = activate(s);
   if (rc) return rc;
   TB_CU("cuStreamBeginCapture", driver()->cuStreamBeginCapture_v2(st->raw, CU_STREAM_CAPTURE_MODE_THREAD_LOCAL));
+  st->capture = capture_id(st);
   return TB_OK;
 }
 
@@ -52,7 +54,8 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
   if (rc) return rc;
   const DriverApi* d = driver();
   CUgraph graph = nullptr;
-  const unsigned long long id = capture_id(st);
+  const unsigned long long id = st->capture;  // (an invalidated capture has lost its id in the driver)
+  st->capture = 0;
   std::vector<CUdeviceptr> work = id ? take_captured_work(s, id) : std::vector<CUdeviceptr>();
   const auto drop_work = [&] {
     for (CUdeviceptr p : work) d->cuMemFree_v2(p);
@@ -74,6 +77,7 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
   g->session = s;
   g->exec = exec;
   g->work = std::move(work);
+  g->work_epoch = s->work_epoch.load();
   s->refs.fetch_add(1);
   *out = reinterpret_cast<tb_graph_exec*>(g);
   return TB_OK;
@@ -89,6 +93,9 @@ tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_str
   if (rc) return rc;
   rc = activate(s);
   if (rc) return rc;
+  if (const uint64_t epoch = s->work_epoch.load(); !g->work.empty() && g->work_epoch.exchange(epoch) != epoch)
+    for (CUdeviceptr p : g->work)
+      if ((rc = clear_counters(st, p))) return rc;
   TB_CU("cuGraphLaunch", driver()->cuGraphLaunch(g->exec, st->raw));
   return TB_OK;
 }

@@ -57,7 +57,9 @@ struct Stream : RefCounted {
   // that a second host thread on the stream cannot replace it in between.
   CUdeviceptr work = 0;
   size_t work_bytes = 0;
+  uint64_t work_epoch = 0;  // Session::work_epoch when its counters were last known to be zero
   std::mutex enqueue;
+  unsigned long long capture = 0;  // the driver's id of the capture that tb_capture_begin began
 };
 
 // Workspace that operators took while their stream was being captured: it belongs to the
@@ -113,6 +115,8 @@ struct Session : RefCounted {
   std::unordered_map<CUfunction, int> pair_occupancy;  // resident CTA pairs of a built-in pair kernel
   std::unordered_set<void*> pinned;
   std::vector<CapturedWork> captured_work;  // of captures that have not ended
+  // Raised when a kernel reports that it gave up a wait: its workspace's counters may not be zero.
+  std::atomic<uint64_t> work_epoch{0};
   StatusWord status;
   int sm_count = 0;
   int max_smem_optin = 0;
@@ -133,6 +137,8 @@ tb_status stream_scratch(Session* s, Stream* st, size_t bytes, CUdeviceptr* out)
 // At least `bytes` of zeroed-at-first workspace for an operator on the stream: the stream's
 // own, or, while the stream is being captured, memory of the graph. The caller holds st->enqueue.
 tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* out);
+// Zeroes the counters at a workspace's front, in stream order.
+tb_status clear_counters(Stream* st, CUdeviceptr work);
 // The id of the capture that `st` is part of, 0 outside a capture.
 unsigned long long capture_id(Stream* st);
 // Takes the workspaces of an ended capture out of the session's list.

@@ -12,6 +12,8 @@
 namespace tb {
 namespace {
 
+constexpr uint64_t kMaxBatch = 1ull << 30;
+
 struct AttnAttrs {
   bool causal = false;
   double scale = 0.0;  // 0: 1/sqrt(D)
@@ -21,6 +23,7 @@ struct AttnAttrs {
 
 tb_status parse_attrs(const tb_attr* attrs, uint32_t n, const char* op, bool paged, AttnAttrs* out) {
   out->causal = paged;
+  if (n && !attrs) return contract(std::string(op) + " attributes are null");
   for (uint32_t i = 0; i < n; ++i) {
     const char* key = attrs[i].key ? attrs[i].key : "";
     if (strcmp(key, "causal") == 0 && !attrs[i].str && attrs[i].value >= 0 && attrs[i].value <= 1) {
@@ -58,7 +61,7 @@ tb_status query_side(const char* op, const tb_tensor* q, const tb_tensor* output
     if (output->shape[a] != q->shape[a]) return contract(name + " output shape mismatch");
   const uint64_t T = q->shape[0], H = q->shape[1], D = q->shape[2];
   if (T == 0 || H == 0 || D == 0) return contract(name + " requires non-zero T, H, and D dimensions");
-  if (T > 0x7fffffffull || H > 0xffffull) return contract(name + " shape exceeds i32 ABI");
+  if (T > (uint64_t)kMaxRows || H > 0xffffull) return contract(name + " shape exceeds i32 ABI");
   if (D > 256) return unsupported(name + " does not implement head dimensions above 256");
   if (!distinct_elements(output)) return contract(name + " requires an output whose elements do not overlap");
   c->dtype = q->dtype;
@@ -234,7 +237,7 @@ using namespace tb;
 extern "C" tb_status tb_op_attention_varlen(tb_session* session, tb_stream* stream, const tb_tensor* q,
                                             const tb_tensor* k, const tb_tensor* v, const tb_tensor* cu_seqlens_q,
                                             const tb_tensor* cu_seqlens_k, const tb_tensor* output,
-                                            const tb_attr* attrs, uint32_t num_attrs, tb_event** out) {
+                                            const tb_attr* attrs, uint32_t num_attrs, tb_event** out) try {
   static const char* const op = "attention.varlen";
   Session* s = reinterpret_cast<Session*>(session);
   if (!q || !k || !v || !cu_seqlens_q || !output)
@@ -249,14 +252,14 @@ extern "C" tb_status tb_op_attention_varlen(tb_session* session, tb_stream* stre
   for (int i = 0; i < 3; ++i)
     if (k->shape[i] != v->shape[i]) return contract("attention.varlen requires K and V of one shape");
   if (k->shape[0] == 0) return contract("attention.varlen requires non-zero T, H, and D dimensions");
-  if (k->shape[0] > 0x7fffffffull) return contract("attention.varlen shape exceeds i32 ABI");
+  if (k->shape[0] > (uint64_t)kMaxRows) return contract("attention.varlen shape exceeds i32 ABI");
   if (k->shape[2] != (uint64_t)c.p.dim) return contract("attention.varlen requires Q, K, and V of one head dimension");
   if ((rc = heads_match(op, k->shape[1], &c))) return rc;
   if (!cu_seqlens_k && k->shape[0] != q->shape[0])
     return contract("attention.varlen requires cu_seqlens_k when Q and K have different row counts");
   const tb_tensor* cu_k = cu_seqlens_k ? cu_seqlens_k : cu_seqlens_q;
   if (!is_index(cu_seqlens_q, 1) || !is_index(cu_k, 1) || cu_seqlens_q->shape[0] < 2 ||
-      cu_seqlens_q->shape[0] > 0x7fffffffull || cu_k->shape[0] != cu_seqlens_q->shape[0])
+      cu_seqlens_q->shape[0] > kMaxBatch + 1 || cu_k->shape[0] != cu_seqlens_q->shape[0])
     return contract("attention.varlen requires contiguous I32 cu_seqlens of one length, batch + 1");
   if (!s) return set_error(TB_ERR_INVALID, "contract", "null session");
   Stream* st = nullptr;
@@ -281,13 +284,15 @@ extern "C" tb_status tb_op_attention_varlen(tb_session* session, tb_stream* stre
   c.p.batch = (int32_t)cu_seqlens_q->shape[0] - 1;
   if ((rc = run_attention(s, st, op, &c, a))) return rc;
   return record_event(s, st, nullptr, out);
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
 extern "C" tb_status tb_op_attention_paged(tb_session* session, tb_stream* stream, const tb_tensor* q,
                                            const tb_tensor* k_cache, const tb_tensor* v_cache,
                                            const tb_tensor* block_table, const tb_tensor* seq_lens,
                                            const tb_tensor* cu_seqlens_q, const tb_tensor* output,
-                                           const tb_attr* attrs, uint32_t num_attrs, tb_event** out) {
+                                           const tb_attr* attrs, uint32_t num_attrs, tb_event** out) try {
   static const char* const op = "attention.paged";
   Session* s = reinterpret_cast<Session*>(session);
   if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !cu_seqlens_q || !output)
@@ -309,7 +314,7 @@ extern "C" tb_status tb_op_attention_paged(tb_session* session, tb_stream* strea
     return contract("attention.paged requires Q, K, and V of one head dimension");
   if ((rc = heads_match(op, k_cache->shape[2], &c))) return rc;
   const uint64_t batch = seq_lens->rank == 1 ? seq_lens->shape[0] : 0;
-  if (!is_index(seq_lens, 1) || !is_index(cu_seqlens_q, 1) || batch == 0 || batch >= 0x7fffffffull ||
+  if (!is_index(seq_lens, 1) || !is_index(cu_seqlens_q, 1) || batch == 0 || batch > kMaxBatch ||
       cu_seqlens_q->shape[0] != batch + 1)
     return contract("attention.paged requires contiguous I32 seq_lens [batch] and cu_seqlens_q [batch + 1]");
   if (!is_index(block_table, 2) || block_table->shape[0] != batch || block_table->shape[1] == 0 ||
@@ -346,4 +351,6 @@ extern "C" tb_status tb_op_attention_paged(tb_session* session, tb_stream* strea
   c.p.width = (int32_t)block_table->shape[1];
   if ((rc = run_attention(s, st, op, &c, a))) return rc;
   return record_event(s, st, nullptr, out);
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }

@@ -21,7 +21,7 @@ bool same_rows(const tb_tensor* rows, const tb_tensor* cache) {
 
 extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, const tb_tensor* k, const tb_tensor* v,
                                      const tb_tensor* slot_map, const tb_tensor* k_cache, const tb_tensor* v_cache,
-                                     const tb_attr* attrs, uint32_t num_attrs, tb_event** out) {
+                                     const tb_attr* attrs, uint32_t num_attrs, tb_event** out) try {
   (void)attrs;
   Session* s = reinterpret_cast<Session*>(session);
   if (!k || !v || !slot_map || !k_cache || !v_cache)
@@ -95,16 +95,19 @@ extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, con
   void* params[] = {&p};
   if ((rc = launch_overlapped(s, st, fn, (unsigned)grid, 1, kAppendThreads, 0, params, entry))) return rc;
   return record_event(s, st, nullptr, out);
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
 extern "C" tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const tb_tensor* context_lens,
                                    const tb_tensor* new_lens, const tb_tensor* free_pages, const tb_tensor* block_table,
                                    const tb_tensor* seq_lens, const tb_tensor* cu_seqlens, const tb_tensor* slot_map,
-                                   const tb_tensor* status, const tb_attr* attrs, uint32_t num_attrs, tb_event** out) {
+                                   const tb_tensor* status, const tb_attr* attrs, uint32_t num_attrs, tb_event** out) try {
   Session* s = reinterpret_cast<Session*>(session);
   if (!context_lens || !new_lens || !free_pages || !block_table || !seq_lens || !cu_seqlens || !slot_map || !status)
     return contract("kv_cache.plan requires context_lens, new_lens and free_pages, and the outputs block_table, "
                     "seq_lens, cu_seqlens, slot_map and status");
+  if (num_attrs && !attrs) return contract("kv_cache.plan attributes are null");
   for (uint32_t i = 0; i < num_attrs; ++i)
     if (!attrs[i].key || strcmp(attrs[i].key, "page_size") != 0)
       return unsupported("kv_cache.plan does not implement attributes other than page_size");
@@ -122,7 +125,8 @@ extern "C" tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const
       block_table->shape[0] != B)
     return contract("kv_cache.plan requires [batch] lengths, a [batch + 1] cu_seqlens and a [batch, pages] block_table");
   if (status->shape[0] != 2) return contract("kv_cache.plan requires a status of two words");
-  if (W > 0x7fffffffull || T > 0x7fffffffull || F > 0x7fffffffull) return contract("kv_cache.plan shape exceeds i32 ABI");
+  // (The kernel steps over tokens and table entries in 32 bits.)
+  if (W > 0x7f000000ull || T > 0x7f000000ull || F > 0x7fffffffull) return contract("kv_cache.plan shape exceeds i32 ABI");
   if (B > kMaxPlanRequests) return unsupported("kv_cache.plan does not implement batches above 16384 requests");
   if (!distinct_elements(block_table)) return contract("kv_cache.plan requires a block_table whose rows do not overlap");
   if (!s) return set_error(TB_ERR_INVALID, "contract", "null session");
@@ -180,4 +184,6 @@ extern "C" tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const
                               entry)))
     return rc;
   return record_event(s, st, nullptr, out);
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }

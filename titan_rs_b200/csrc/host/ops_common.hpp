@@ -2,6 +2,7 @@
 // runtime's messages, attribute lookup, tensor-map encoding and launches.
 #pragma once
 
+#include <exception>
 #include <string>
 
 #include "internal.hpp"
@@ -52,6 +53,9 @@ inline uint64_t numel(const tb_tensor* t) {
 
 inline tb_status contract(const std::string& msg) { return set_error(TB_ERR_INVALID, "contract", msg); }
 inline tb_status unsupported(const std::string& msg) { return set_error(TB_ERR_UNSUPPORTED, "contract", msg); }
+
+// What a C entry answers for a C++ exception (memory for a string or a list ran out).
+inline tb_status caught(const std::exception& e) { return set_error(TB_ERR_OUT_OF_MEMORY, "allocate", e.what()); }
 
 inline const tb_attr* find_attr(const tb_attr* attrs, uint32_t n, const char* key) {
   for (uint32_t i = 0; i < n; ++i)

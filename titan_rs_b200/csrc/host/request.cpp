@@ -35,11 +35,13 @@ extern "C" {
 
 tb_status tb_request_create(tb_session* session, tb_stream* stream, const char* op, const tb_tensor* inputs,
                             uint32_t num_inputs, const tb_tensor* outputs, uint32_t num_outputs, const tb_attr* attrs,
-                            uint32_t num_attrs, tb_request** out) {
+                            uint32_t num_attrs, tb_request** out) try {
   Session* s = reinterpret_cast<Session*>(session);
   if (!out || !op || (num_inputs && !inputs) || (num_outputs && !outputs) || (num_attrs && !attrs))
     return contract("a request needs an operator name, its tensors and a place for the handle");
   if (!s) return set_error(TB_ERR_INVALID, "contract", "null session");
+  if (num_inputs > 64 || num_outputs > 64 || num_attrs > 64)
+    return contract("a request takes up to 64 inputs, outputs and attributes each");
   Stream* st = nullptr;
   tb_status rc = check_stream(s, stream, &st);
   if (rc) return rc;
@@ -67,6 +69,8 @@ tb_status tb_request_create(tb_session* session, tb_stream* stream, const char* 
     for (const tb_tensor& t : *list) tb_buffer_retain(t.buffer);
   *out = reinterpret_cast<tb_request*>(r);
   return TB_OK;
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
 tb_status tb_request_enqueue(const tb_request* request, tb_event** out) {

@@ -101,6 +101,9 @@ TB_INDEX_FN int load_index(const int* p) { return __ldg(p); }
 TB_INDEX_FN int load_index(const int* p) { return *p; }
 #endif
 
+// Rows of one tensor, and keys of one request, at most: sums with a tile's rows stay below 2^31.
+constexpr int64_t kMaxRows = 0x7fffff00;
+
 // Request b: its query rows [q0, q0 + lq) and its keys (lk of them, from row k0 when packed).
 struct AttnRequest {
   int q0, lq, k0, lk;
@@ -116,7 +119,7 @@ TB_INDEX_FN AttnRequest request_of(const AttnParams& p, int b) {
   if (p.table) {
     const int64_t most = (int64_t)p.width * p.page;
     r.k0 = 0;
-    r.lk = clamp_index(load_index(reinterpret_cast<const int*>(p.lens) + b), 0, most);
+    r.lk = clamp_index(load_index(reinterpret_cast<const int*>(p.lens) + b), 0, most < kMaxRows ? most : kMaxRows);
   } else {
     const int* cu_k = reinterpret_cast<const int*>(p.cu_k);
     r.k0 = clamp_index(load_index(cu_k + b), 0, p.tk);
