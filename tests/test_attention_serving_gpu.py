@@ -331,6 +331,42 @@ def test_paged_cache_with_heads_before_rows(session, rt):
     assert_attention(got.outputs[0].to_numpy(rt.stream), ref, mag, dtype, 333, np.nanmax(np.abs(as_f64(v))))
 
 
+@pytest.mark.parametrize("candidate", ["attention_rows", "attention_tiles"])
+@pytest.mark.parametrize("dtype,d", [(DType.BF16, 128), (DType.F16, 64)])
+def test_each_candidate_takes_chunks(session, rt, candidate, dtype, d):
+    name = check_varlen(session, rt, [130, 0, 1, 300], [64, 9, 500, 333], 8, 2, d, dtype, True, pad=2, seed=560,
+                        candidate=candidate)
+    assert name.startswith(candidate)
+    name = check_paged(session, rt, [200, 333, 1200, 40], [200, 130, 1, 0], 8, 2, d, 16, dtype, pad=3, seed=570,
+                       attrs={"candidate": candidate})
+    assert name.startswith(candidate)
+
+
+@pytest.mark.parametrize("candidate", ["attention_rows", "attention_tiles", "attention_tokens"])
+def test_each_candidate_takes_single_tokens(session, rt, candidate):
+    name = check_paged(session, rt, [700, 1, 65, 0], [1, 1, 1, 1], 8, 2, 128, 32, DType.BF16, pad=1, seed=580,
+                       attrs={"candidate": candidate, "max_query_len": 1})
+    assert name.startswith(candidate)
+
+
+def test_the_default_kernel_follows_shapes_and_bounds(session, rt):
+    one = dict(lens=[300, 20], new=[1, 1], h=8, hk=2, d=128, dtype=DType.BF16)
+    assert check_paged(session, rt, page=16, attrs={"max_query_len": 1}, **one) == "attention_tokens_bf16_d128_r8"
+    assert check_paged(session, rt, page=24, attrs={"max_query_len": 8}, **one) == "attention_tokens_bf16_d128_r8"
+    few = {**one, "new": [4, 1]}
+    assert check_paged(session, rt, page=24, attrs={"max_query_len": 4}, **few) == "attention_tokens_bf16_d128_r16"
+    few = {**one, "new": [8, 3]}
+    assert check_paged(session, rt, page=16, attrs={"max_query_len": 8}, **few) == "attention_tokens_bf16_d128_r32"
+    long = dict(lens=[300, 60], new=[1, 40], h=8, hk=2, d=64, dtype=DType.F16)
+    assert check_paged(session, rt, page=16, **long) == "attention_tiles_f16_d64"
+    assert check_paged(session, rt, page=24, **long) == "attention_rows_f16"
+    assert check_varlen(session, rt, [30], None, 4, 4, 128, DType.BF16, True) == "attention_tiles_bf16_d128"
+    assert check_varlen(session, rt, [30], None, 4, 4, 96, DType.BF16, True) == "attention_rows_bf16"
+    for attrs in ({"candidate": "attention_tokens"}, {"candidate": "attention_tiles"}):
+        with pytest.raises(tb.ExecutionError, match="does not take"):
+            check_paged(session, rt, page=24, attrs=attrs, **long)
+
+
 def test_unknown_candidate_foreign_session_and_small_buffers(session, rt):
     q = upload(session, rt.stream, rows((4, 2, 64), DType.BF16, 1), DType.BF16)
     cu = ints(session, rt, [0, 4])

@@ -206,21 +206,23 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
   if (rc) return rc;
   c->p.causal = a.causal ? 1 : 0;
   c->p.scale = (float)(a.scale > 0.0 ? a.scale : 1.0 / std::sqrt((double)c->p.dim));
-  const bool only_rows = a.candidate && strcmp(a.candidate, "attention_rows") == 0;
-  const bool only_tiles = a.candidate && strcmp(a.candidate, "attention_tiles") == 0;
-  if (a.candidate && !only_rows && !only_tiles)
-    return contract(std::string("unknown ") + op + " candidate " + a.candidate);
-  const bool tiles = !only_rows && tiles_fit(c->p);
-  if (only_tiles && !tiles)
-    return unsupported("candidate attention_tiles does not take this shape, page size or alignment");
-  std::lock_guard<std::mutex> lock(st->enqueue);
+  const std::string only = a.candidate ? a.candidate : "";
+  if (!only.empty() && only != "attention_rows" && only != "attention_tiles" &&
+      !(c->p.table && only == "attention_tokens"))
+    return contract(std::string("unknown ") + op + " candidate " + only);
   const uint64_t group = (uint64_t)(c->p.heads / c->p.kv_heads);
   const uint64_t longest = a.max_query && a.max_query < (uint64_t)c->p.tq ? a.max_query : (uint64_t)c->p.tq;
-  const bool tokens = c->p.table && !a.candidate && rows_aligned(c->p);
-  // A step whose requests all have few rows (the caller's bound says so) is the token kernel's.
-  // Other steps take one launch of the tile kernel, which reads single tokens' keys at 100 us
-  // for 64 requests of 300-8192 keys beside chunks (a launch of each kernel costs more).
-  const bool few = tokens && longest * group <= 32;
+  const bool tiles = tiles_fit(c->p) && (only.empty() || only == "attention_tiles");
+  const bool tokens = c->p.table && rows_aligned(c->p) && (only.empty() || only == "attention_tokens");
+  const bool few = tokens && longest * group <= 32;  // every request has few rows: the caller's bound says so
+  if ((only == "attention_tiles" && !tiles) || (only == "attention_tokens" && !few))
+    return unsupported("candidate " + only + " does not take this shape, page size, alignment or max_query_len");
+  std::lock_guard<std::mutex> lock(st->enqueue);
+  // Steps of few rows are the token kernel's. Other steps take one launch of the tile kernel for
+  // all requests: it reads single tokens' keys more slowly (64 requests of 300-8192 keys 128 us
+  // against 110, four of 110-131 thousand 600 against 334), but a launch of each kernel costs
+  // more where chunks fill the step (eight requests, two of them single tokens, 150 us
+  // against 124). Where tiles do not fit, the token kernel still takes the single tokens.
   if (few || (tokens && !tiles && group <= 32)) {
     const uint64_t rows = few ? longest * group : group;
     c->p.token_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
