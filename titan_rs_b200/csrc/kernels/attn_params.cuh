@@ -84,18 +84,20 @@ constexpr int kTileBarrierBytes = 512, kTileScratchBytes = 512;
 TB_BOTH constexpr int tile_smem_bytes(int dim) {
   return 7 * 128 * dim * 2 + kTileBarrierBytes + kTileScratchBytes + 1024;
 }
+
 // The index arithmetic is shared by the kernels and a host test of it.
 #ifdef __CUDACC__
 // These kernels are launched with programmatic stream serialization (launch_overlapped):
 // the next one's blocks are set up while the one before still runs. Every thread calls this
 // before its first access to global memory; it returns when the grids before have ended and
-// their writes are visible.
+// their writes are visible. (To plain loads: what an earlier grid wrote is not read through
+// the read-only path, whose data has to be constant for a grid's whole life.)
 __device__ __forceinline__ void begin_after_earlier_grids() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 #define TB_INDEX_FN __device__ __forceinline__
-TB_INDEX_FN int load_index(const int* p) { return __ldg(p); }
+TB_INDEX_FN int load_index(const int* p) { return *p; }
 #else
 #define TB_INDEX_FN inline
 TB_INDEX_FN int load_index(const int* p) { return *p; }

@@ -35,7 +35,7 @@ __device__ __forceinline__ void attention_rows(const AttnParams& p) {
     int lo = 0, hi = p.batch;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(cu_q + mid) <= t) lo = mid + 1;
+      if (load_index(cu_q + mid) <= t) lo = mid + 1;
       else hi = mid;
     }
     if (lo == 0) continue;

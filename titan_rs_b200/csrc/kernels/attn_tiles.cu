@@ -25,7 +25,14 @@
 //                then come requests with more than half of a share, a quarter, and the rest,
 //                so that no long item starts when the others are done. The warpgroup that
 //                finishes a tile's last part adds the parts up, in their order.
-// Bound by the softmax and the single issuing lane beside the tensor core, as the square kernel.
+// Bound by the chain of a tile's softmax and products: a step of the steady state takes about
+// 3,360 cycles, of which the tensor core works 2,176 and a tile's exponentials 2,048; an item
+// adds some 4,000 in which its rows are stored. Eight prompts of 4096 tokens (1.1 TFLOP under
+// the mask) take 1,000 us with 32 key heads and 959 with 8 (burst; 985 and 944 in a long run),
+// 1.10 and 1.15 PFLOP/s against 1.05 of the square kernel. Built and not kept: two threads a row
+// (sixteen softmax warps, 1,110 us: agreeing on the row's maximum costs more than the halves
+// save), K and V asked into L2 a tile ahead (8% slower: the copy engine takes each
+// request in turn), the same for the next item's first tiles (7%).
 // Every wait is bounded; on a timeout the kernel records a code, drains and returns.
 #include <cuda_fp16.h>
 
@@ -54,7 +61,7 @@ static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kTileThreads * kTileLau
 constexpr int kSlots = 4;         // item descriptions in flight
 constexpr int kItemReaders = 11;  // warps 0, 1, 2 and the eight softmax warps
 constexpr int kQ = 3;             // Q tiles in shared memory
-constexpr long long kGroupBytes = 32ll << 20;  // K and V that are worked on at a time
+constexpr long long kGroupBytes = 32ll << 20;  // K and V worked on at a time (909 us for long prompts; 921 without)
 
 struct Barriers {
   uint64_t q_full[kQ], q_empty[kQ];
@@ -145,7 +152,8 @@ __device__ __forceinline__ int key_tiles(const AttnRequest& r) { return (r.lk + 
 // memory), so it has to save more.
 __device__ __forceinline__ int class_of(const AttnParams& p, const AttnRequest& r, long long share) {
   const int n = key_tiles(r);
-  return p.cut && n > share + share / 8 + 6 ? 0 : n > share ? 1 : 2 * n > share ? 1 : 4 * n > share ? 2 : 3;
+  if (p.cut && n > share + share / 8 + 6) return 0;
+  return 2 * n > share ? 1 : 4 * n > share ? 2 : 3;
 }
 
 __device__ __forceinline__ int parts_of(const AttnRequest& r, long long share) {

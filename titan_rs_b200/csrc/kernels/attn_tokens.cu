@@ -33,7 +33,9 @@ constexpr int kTile = kTokenTile;  // 16 keys a warp
 constexpr int kThreads = kTokenThreads;
 constexpr int kStages = kTokenStages;
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kMinRun = 2;  // tiles of a CTA at least, where there are so many (11.3 us for 1018 keys x 8 heads; 12.5 with 1, 12.7 with 4)
+// Tiles of a CTA at least, where there are so many (11.3 us for 1018 keys of eight heads; 12.5
+// with one, 12.7 with four).
+constexpr int kMinRun = 2;
 
 template <int D>
 TB_BOTH constexpr int stage_bytes() { return 2 * kTile * D * 2; }
@@ -284,8 +286,8 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t* at = reinterpret_cast<const uint32_t*>(q + k * 16 + (lane & 3) * 2);
-          qf[t][k][0] = in ? __ldg(at) : 0u;
-          qf[t][k][1] = in ? __ldg(at + 4) : 0u;
+          qf[t][k][0] = in ? at[0] : 0u;
+          qf[t][k][1] = in ? at[4] : 0u;
         }
       }
     }

@@ -35,7 +35,7 @@ __device__ __forceinline__ void append_rows(const AppendParams& p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool in = t + i * step < p.tokens;
-        slot[i] = in ? __ldg(slots + t + i * step) : -1;
+        slot[i] = in ? slots[t + i * step] : -1;
         if (in) x[i] = *reinterpret_cast<const Chunk*>(from + (t + i * step) * r_tok);
       }
 #pragma unroll
@@ -102,11 +102,11 @@ __device__ __forceinline__ void plan_step(const PlanParams& p) {
   const int lo = min((int)threadIdx.x * per, p.batch), hi = min(lo + per, p.batch);
   const auto pages = [&](long long tokens) { return (tokens + p.page - 1) / p.page; };
   long long tokens = 0, total = 0;
-  for (int b = lo; b < hi; ++b) tokens += max(__ldg(add + b), 0);
+  for (int b = lo; b < hi; ++b) tokens += max(add[b], 0);
   long long at = sum_before<kThreads>(tokens, sums[0], total);
   long long need = 0;
   for (int b = lo; b < hi; ++b) {
-    const long long c = __ldg(ctx + b), n = __ldg(add + b);
+    const long long c = ctx[b], n = add[b];
     const bool fits = c >= 0 && n >= 0 && c + n <= 0x7fffffff && pages(c + n) <= p.width && at + n <= p.tokens;
     const int own = fits ? (int)(pages(c + n) - pages(c)) : -1;
     start[b] = (int)min(at, (long long)p.tokens);
@@ -139,17 +139,17 @@ __device__ __forceinline__ void plan_step(const PlanParams& p) {
   for (int b = tid; b <= p.batch; b += threads) {
     reinterpret_cast<int*>(p.cu)[b] = start[b];
     if (b < p.batch) {
-      const int c = max(__ldg(ctx + b), 0);
-      reinterpret_cast<int*>(p.lens)[b] = first[b] >= 0 ? c + __ldg(add + b) : c;
+      const int c = max(ctx[b], 0);
+      reinterpret_cast<int*>(p.lens)[b] = first[b] >= 0 ? c + add[b] : c;
     }
   }
   // The new entries of the table, a warp a request.
   for (int b = tid >> 5; b < p.batch; b += threads >> 5) {
     if (first[b] < 0) continue;
-    const long long c = __ldg(ctx + b);
-    const int held = (int)pages(c), wanted = (int)pages(c + __ldg(add + b));
+    const long long c = ctx[b];
+    const int held = (int)pages(c), wanted = (int)pages(c + add[b]);
     for (int i = held + (int)(threadIdx.x & 31); i < wanted; i += 32)
-      table[b * p.table_row + i] = __ldg(free_pages + first[b] + i - held);
+      table[b * p.table_row + i] = free_pages[first[b] + i - held];
   }
   for (int t = tid; t < p.tokens; t += threads) {
     int below = 0, above = p.batch + 1;  // the last request that starts at or before token t
@@ -161,8 +161,8 @@ __device__ __forceinline__ void plan_step(const PlanParams& p) {
     const int b = below - 1;
     int slot = -1;
     if (b < p.batch && first[b] >= 0) {
-      const int c = __ldg(ctx + b), x = c + t - start[b], index = x / p.page, held = (int)pages(c);
-      const int id = index < held ? table[b * p.table_row + index] : __ldg(free_pages + first[b] + index - held);
+      const int c = ctx[b], x = c + t - start[b], index = x / p.page, held = (int)pages(c);
+      const int id = index < held ? table[b * p.table_row + index] : free_pages[first[b] + index - held];
       const long long place = (long long)id * p.page + x % p.page;
       if (id >= 0 && place <= 0x7fffffff) slot = (int)place;
     }

@@ -161,14 +161,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-__device__ __forceinline__ void tma_prefetch_l2_4d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
-                                                   int32_t w) {
-  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y), "r"(z), "r"(w)
-               : "memory");
-}
-
 // ------------------------------------------------------------------ tcgen05 / TMEM
 // Allocation is warp-wide: all 32 lanes of one warp execute it.
 __device__ __forceinline__ void tmem_alloc(uint32_t* result_smem, uint32_t ncols) {
