@@ -192,7 +192,7 @@ tb_status launch_tokens(Session* s, Stream* st, AttnCall* c) {
   CUfunction fn = nullptr;
   tb_status rc = builtin_function(s, "attn_tokens", entry.c_str(), &fn);
   if (rc) return rc;
-  const int ctas = std::min(2 * s->sm_count, kTokenMaxCtas);  // two resident on each SM
+  const int ctas = std::min(token_per_sm(c->p.token_rows) * s->sm_count, kTokenMaxCtas);
   CUdeviceptr work = 0;
   if ((rc = stream_workspace(s, st, token_workspace_bytes(ctas, c->p.token_rows, c->p.dim), &work))) return rc;
   c->p.work = work;
@@ -220,7 +220,7 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
   std::lock_guard<std::mutex> lock(st->enqueue);
   // Steps of few rows are the token kernel's. Other steps take one launch of the tile kernel for
   // all requests: it reads single tokens' keys more slowly (64 requests of 300-8192 keys 128 us
-  // against 110, four of 110-131 thousand 600 against 334), but a launch of each kernel costs
+  // against 97, four of 110-131 thousand 600 against 304), but a launch of each kernel costs
   // more where chunks fill the step (eight requests, two of them single tokens, 150 us
   // against 124). Where tiles do not fit, the token kernel still takes the single tokens.
   if (few || (tokens && !tiles && group <= 32)) {

@@ -57,13 +57,16 @@ TB_BOTH constexpr uint64_t token_workspace_bytes(int ctas, int rows, int dim) {
   return kWorkFront + 2ull * ctas * token_slot_floats(rows, dim) * 4;
 }
 
-// The token kernel: keys of a tile, stages of its ring, and its shared memory (the ring, the
-// row offsets of three tiles, two Q blocks where they fit (16 rows), the joined statistics
-// and some words; 128 bytes to align).
-constexpr int kTokenTile = 64, kTokenStages = 3, kTokenThreads = 128;
+// The token kernel: keys of a tile, and, for eight rows and for more, stages of the ring and CTAs
+// of an SM (registers allow three only with eight rows), and its shared memory (the ring, the
+// row offsets of each stage, two Q blocks where they fit (16 rows), the joined statistics and
+// some words; 128 bytes to align).
+constexpr int kTokenTile = 64, kTokenThreads = 128;
+TB_BOTH constexpr int token_stages(int rows) { return rows <= 8 ? 2 : 3; }
+TB_BOTH constexpr int token_per_sm(int rows) { return rows <= 8 ? 3 : 2; }
 TB_BOTH constexpr int token_smem_bytes(int dim, int rows) {
-  return kTokenStages * (2 * kTokenTile * dim * 2 + kTokenTile * 16) + (rows <= 16 ? 2 * rows * dim * 2 : 0) +
-         2 * 4 * 8 * 4 + 256 + 128;
+  return token_stages(rows) * (2 * kTokenTile * dim * 2 + kTokenTile * 16) + (rows <= 16 ? 2 * rows * dim * 2 : 0) +
+         2 * (kTokenThreads / 32) * 8 * 4 + 256 + 128;
 }
 
 // The tile kernel's workspace for the parts of items whose keys are cut, in slots of 256 rows,

@@ -5,7 +5,7 @@
 // Every cached row is read once for the G x Lq (query row, head) pairs of its key head, so at
 // 2 G Lq flops a byte the kernel is bound by the HBM, and the design serves the loads:
 //   - One list of 64-key tiles over all (request, key head) pairs is cut into equal runs, one
-//     per CTA (two CTAs an SM), so requests of any lengths load the SMs evenly. A pair that
+//     per resident CTA, so requests of any lengths load the SMs evenly. A pair that
 //     is cut leaves partial results (O, m, sum) in the workspace; the CTA that finishes it
 //     last adds them up in the order of the runs, so the result does not depend on who is last.
 //   - Tiles arrive in a ring of shared-memory stages by 16-byte cp.async, which takes any
@@ -17,6 +17,12 @@
 //     columns (a tcgen05 tile has 64 or 128 rows, of which a decode step would fill 8). Each
 //     warp takes 16 keys of a tile with a maximum and sum of its own, so the warps
 //     meet only for the stage hand-over; they are joined when the pair ends.
+//   - Three CTAs an SM with two stages each where the query rows are eight or fewer, two with three
+//     stages where more rows take the registers. What bounds a tile's step is the latency of its
+//     chain (wait, first product, softmax, second product) and not the depth of the ring, so more
+//     warps help and fewer do not: 64 requests of 300-8192 keys (544 MB) 97 us against 108
+//     with two CTAs of three stages, 131 with three of 32-key tiles and 127 with one of 128-key
+//     tiles; four of 110-131 thousand (2.0 GB) 304 us, 6.6 TB/s, against 330.
 // Scores, statistics and O are fp32; P is rounded to the values' type for the second product
 // (at most 2^8: the reference maximum moves only when a row's maximum grows by more than 2^8).
 #include <cuda_bf16.h>
@@ -31,10 +37,11 @@ using namespace tb;
 
 constexpr int kTile = kTokenTile;  // 16 keys a warp
 constexpr int kThreads = kTokenThreads;
-constexpr int kStages = kTokenStages;
+constexpr int kWarps = kThreads / 32;
+static_assert(kTile == 16 * kWarps && kThreads > kTile, "a warp takes 16 keys of a tile, a thread looks a row up");
 constexpr float kLowest = -3.402823466e38f;
-// Tiles of a CTA at least, where there are so many (11.3 us for 1018 keys of eight heads; 12.5
-// with one, 12.7 with four).
+// Tiles of a CTA at least, where there are so many (11.4 us for 1018 keys of eight heads; 14.0
+// with three, 13.2 with four).
 constexpr int kMinRun = 2;
 
 template <int D>
@@ -153,10 +160,11 @@ struct PairRows {
 
 template <int D, int kRows>
 struct Shared {
+  static constexpr int kStages = token_stages(kRows);
   alignas(128) uint8_t stage[kStages][stage_bytes<D>()];  // K rows, then V rows; 16-byte chunks swizzled by row
   alignas(16) uint8_t q[kRows <= 16 ? 2 : 0][kRows * D * 2 + (kRows <= 16 ? 0 : 16)];
   TileRows at[kStages];
-  float top[4][8], sum[4][8];
+  float top[kWarps][8], sum[kWarps][8];
   PairRows pair[kStages];
   long long scan[kThreads / 32], found_before;
   int found_b, last;
@@ -164,7 +172,7 @@ struct Shared {
 
 template <typename T, int D, int NT>
 __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
-  constexpr int kRows = 8 * NT;
+  constexpr int kRows = 8 * NT, kStages = token_stages(kRows);
   constexpr bool kQShared = kRows <= 16;  // Q comes through shared memory, else by plain loads
   extern __shared__ uint8_t raw[];
   using Smem = Shared<D, kRows>;
@@ -341,7 +349,9 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
 
     // ---- S^T of the warp's 16 keys ----
     const uint32_t ks = smem_of(sm.stage[n % kStages]) + warp * 16 * D * 2, vs = ks + kTile * D * 2;
-    float s[NT][4];
+    // (With one block of columns, two accumulators: a chain of D / 16 products waits for each.)
+    constexpr int kChains = NT == 1 ? 2 : 1;
+    float s[NT][4], other[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -353,14 +363,16 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         uint32_t a[4];
         load_matrix(a, ks + r * (D * 2) + (((k * 2 + (lane >> 4)) ^ (r & 7)) << 4));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) Half<T>::mma(s[t], a, qf[t][k][0], qf[t][k][1]);
+        for (int t = 0; t < NT; ++t) Half<T>::mma(k % kChains ? other : s[t], a, qf[t][k][0], qf[t][k][1]);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[0][i] += other[i];
     }
     // ---- softmax of the columns (query rows) over the warp's keys ----
     const int key = cur.tile * kTile + warp * 16 + (lane >> 2);
     uint32_t pf[NT][2];
     bool grow = false;
-    float mx[NT][2];
+    float mx[NT][2];  // over the thread's own keys: the lanes only meet when a maximum grows
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -368,11 +380,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         if (key + (i >> 1) * 8 >= seen[t][i & 1]) s[t][i] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float x = fmaxf(s[t][i], s[t][i + 2]);
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        mx[t][i] = x * scale2;
+        mx[t][i] = fmaxf(s[t][i], s[t][i + 2]) * scale2;
         grow |= mx[t][i] > top[t][i] + 8.f;
       }
     }
@@ -382,7 +390,10 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float m = fmaxf(top[t][i], mx[t][i]);
+          float m = fmaxf(top[t][i], mx[t][i]);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
           f[i] = exp2_mufu(top[t][i] - m);
           top[t][i] = m;
           sum[t][i] *= f[i];
@@ -417,7 +428,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       }
     }
     if (more) {
-      // (Tile n's offsets were used two iterations ago.)
+      // (Tile n's offsets were used in an earlier iteration.)
       publish(n + kStages, k_next[0], v_next[0], pair);
       ahead.next(p);
     }
@@ -435,13 +446,13 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       const auto place = [&](int row) { return out + (row / group) * p.o_tok + (row % group) * p.o_head; };
       // The tile's stage is free until the next iteration's copies.
       float(*joined)[8][D + 4] = reinterpret_cast<float(*)[8][D + 4]>(sm.stage[n % kStages]);
-      static_assert(sizeof(float) * 4 * 8 * (D + 4) <= stage_bytes<D>(), "joined results fit a stage");
+      static_assert(sizeof(float) * kWarps * 8 * (D + 4) <= stage_bytes<D>(), "joined results fit a stage");
       __syncthreads();
       float* mine_at = slots + (blockIdx.x == first ? 2 * first + 1 : 2 * (long long)blockIdx.x) * slot_floats;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t * 8 >= rows) break;
-        // The four warps' results of eight query rows, joined through shared memory.
+        // The warps' results of eight query rows, joined through shared memory.
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float x = sum[t][i];
@@ -463,11 +474,13 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         const int limit = min(8, rows - t * 8);
         for (int x = tid; x < limit * (D / 4); x += kThreads) {
           const int r = x / (D / 4), d = x % (D / 4) * 4;
-          const float m = fmaxf(fmaxf(sm.top[0][r], sm.top[1][r]), fmaxf(sm.top[2][r], sm.top[3][r]));
+          float m = kLowest;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm.top[w][r]);
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
           float l = 0.f;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < kWarps; ++w) {
             const float f = exp2_mufu(sm.top[w][r] - m);
             add_scaled(acc, *reinterpret_cast<const float4*>(&joined[w][r][d]), f);
             l = fmaf(f, sm.sum[w][r], l);
@@ -524,10 +537,12 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
 
 }  // namespace
 
-#define TB_TOKEN_ENTRY(name, T, D, NT)                                                                       \
-  extern "C" __global__ void __launch_bounds__(kThreads, 2) name(const __grid_constant__ tb::AttnParams p) { \
-    static_assert(sizeof(Shared<D, 8 * NT>) + 128 <= tb::token_smem_bytes(D, 8 * NT), "shared memory reservation");          \
-    attention_tokens<T, D, NT>(p);                                                                           \
+#define TB_TOKEN_ENTRY(name, T, D, NT)                                                       \
+  extern "C" __global__ void __launch_bounds__(kThreads, tb::token_per_sm(8 * NT))           \
+      name(const __grid_constant__ tb::AttnParams p) {                                       \
+    static_assert(sizeof(Shared<D, 8 * NT>) + 128 <= tb::token_smem_bytes(D, 8 * NT),        \
+                  "shared memory reservation");                                              \
+    attention_tokens<T, D, NT>(p);                                                           \
   }
 
 TB_TOKEN_ENTRY(attention_tokens_bf16_d128_r8, __nv_bfloat16, 128, 1)
