@@ -26,13 +26,20 @@
 //                so that no long item starts when the others are done. The warpgroup that
 //                finishes a tile's last part adds the parts up, in their order.
 // Bound by the chain of a tile's softmax and products: a step of the steady state takes about
-// 3,360 cycles, of which the tensor core works 2,176 and a tile's exponentials 2,048; an item
+// 3,300 cycles, of which the tensor core works 2,176 and a tile's exponentials 2,048; an item
 // adds some 4,000 in which its rows are stored. Eight prompts of 4096 tokens (1.1 TFLOP under
-// the mask) take 1,000 us with 32 key heads and 959 with 8 (burst; 985 and 944 in a long run),
-// 1.10 and 1.15 PFLOP/s against 1.05 of the square kernel. Built and not kept: two threads a row
-// (sixteen softmax warps, 1,110 us: agreeing on the row's maximum costs more than the halves
-// save), K and V asked into L2 a tile ahead (8% slower: the copy engine takes each
-// request in turn), the same for the next item's first tiles (7%).
+// the mask) take 976 us with 32 key heads and 935 with 8, 1.13 and 1.18 PFLOP/s against 1.04
+// of the square kernel on the same board.
+// Items of one to four steps are bound by the instruction caches, which the roles' code shares
+// and leaves behind: with the items' arithmetic in 32 bits and the mask, the copies of K and V,
+// the halves of P V and the rows' stores in loops, sixteen ragged prompts went from 125 to 114 us,
+// 24 of dimension 64 over other sequences' keys from 64 to 54, 128 of 256 tokens from 216
+// to 190. Built and not kept: two threads a row (sixteen softmax warps, 1,110 us where one
+// took 992: agreeing on the row's maximum costs more than the halves save), S read from tensor
+// memory a second time for the exponentials (less code, but 4 to 9% slower from four steps on),
+// items drawn earlier where they are short (up to 8% slower: the last ones are spread less
+// evenly), K and V asked into L2 a tile ahead (8% slower: the copy engine takes each request
+// in turn), the same for the next item's first tiles (7%).
 // Every wait is bounded; on a timeout the kernel records a code, drains and returns.
 #include <cuda_fp16.h>
 
@@ -142,7 +149,8 @@ struct Shape {
 
 // Pairs of tiles of one request (0 where the token kernel takes it).
 __device__ __forceinline__ int pairs_of(const AttnParams& p, const AttnRequest& r) {
-  return is_token_request(p, r) ? 0 : (r.lq + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+  if (p.token_rows && is_token_request(p, r)) return 0;
+  return (int)((unsigned)(r.lq + 2 * p.tile_tokens - 1) / (unsigned)(2 * p.tile_tokens));
 }
 
 __device__ __forceinline__ int key_tiles(const AttnRequest& r) { return (r.lk + BN - 1) / BN; }
@@ -150,14 +158,14 @@ __device__ __forceinline__ int key_tiles(const AttnRequest& r) { return (r.lk + 
 // The class of a request: 0 is cut into parts, 1 to 3 are long, middling and short next to
 // a CTA's share. A cut costs a CTA about six key tiles' time (the parts' rows go through
 // memory), so it has to save more.
-__device__ __forceinline__ int class_of(const AttnParams& p, const AttnRequest& r, long long share) {
+__device__ __forceinline__ int class_of(const AttnParams& p, const AttnRequest& r, int share) {
   const int n = key_tiles(r);
   if (p.cut && n > share + share / 8 + 6) return 0;
   return 2 * n > share ? 1 : 4 * n > share ? 2 : 3;
 }
 
-__device__ __forceinline__ int parts_of(const AttnRequest& r, long long share) {
-  return (int)min((long long)kTileMaxParts, (key_tiles(r) + share - 1) / share);
+__device__ __forceinline__ int parts_of(const AttnRequest& r, int share) {
+  return min(kTileMaxParts, (int)((unsigned)(key_tiles(r) + share - 1) / (unsigned)share));
 }
 
 // One 32-column chunk of S to probabilities in the values' type, and its part of the row sum.
@@ -211,7 +219,22 @@ template <typename T, int HD>
 __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, int valid, bool rescale, float scale2,
                                              float& m, float& l, uint64_t* p_half, uint64_t* p_full) {
   const int lane = lane_id();
-  const bool need_mask = valid < BN;
+  // Few tiles have keys to mask: they go through a loop of their own over S in tensor memory.
+  // (Its code four times over in everyone's way took 130 us where this takes 120; sixteen prompts.)
+  if (__any_sync(0xffffffffu, valid < BN)) {
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+      if (__all_sync(0xffffffffu, valid >= c + 32)) continue;
+      uint32_t s[32];
+      tmem_ld_x32(s_tmem + c, s);
+      tmem_ld_wait();
+      reg_fence(s);
+      sdpa2::mask_chunk(s, valid - c);
+      tmem_st_x16(s_tmem + c, reinterpret_cast<uint32_t(&)[16]>(s[0]));
+      tmem_st_x16(s_tmem + c + 16, reinterpret_cast<uint32_t(&)[16]>(s[16]));
+    }
+    tmem_st_wait();
+  }
   uint32_t c0[32], c1[32], c2[32], c3[32];
   tmem_ld_x32(s_tmem, c0);
   tmem_ld_x32(s_tmem + 32, c1);
@@ -223,10 +246,10 @@ __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, i
   reg_fence(c2);
   reg_fence(c3);
   float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  mask_max_chunk(c0, valid, need_mask, mx4);
-  mask_max_chunk(c1, valid - 32, need_mask, mx4);
-  mask_max_chunk(c2, valid - 64, need_mask, mx4);
-  mask_max_chunk(c3, valid - 96, need_mask, mx4);
+  mask_max_chunk(c0, BN, false, mx4);
+  mask_max_chunk(c1, BN, false, mx4);
+  mask_max_chunk(c2, BN, false, mx4);
+  mask_max_chunk(c3, BN, false, mx4);
   const float mx = fmaxf(fmax3f(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale2;
   const bool grow = mx > m + sdpa2::kLazyRescaleLog2;
   if (__any_sync(0xffffffffu, grow)) {
@@ -403,7 +426,9 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < kTileThreads / 32; ++w) total += scratch->sums[w];
-  const long long share = max((long long)kTileMinPart, (total * p.kv_heads + gridDim.x - 1) / gridDim.x);
+  // (Four times a request's key tiles stay below 2^27.)
+  const int share =
+      (int)min(1ll << 27, max((long long)kTileMinPart, (total * p.kv_heads + gridDim.x - 1) / gridDim.x));
   for (int b = threadIdx.x; b < p.batch; b += kTileThreads) {
     const AttnRequest r = request_of(p, b);
     const int c = class_of(p, r, share);
@@ -419,10 +444,12 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     setmaxnreg_dec<kControlRegs>();
     if (warp == 3) {
       // ---------------- items: the longest rows first, drawn from a counter ----------------
-      long long w = blockIdx.x, class_end = 0, before = 0;  // works up to the class's end; units before request b
+      int w = blockIdx.x, class_end = 0, before = 0;  // works up to the class's end; units before request b
       int c = -1, b = 0;                                     // the walk stands in class c before request b
       // (More than max_items only where cu_seqlens counts rows twice; the rest is then left.)
-      const long long most = (long long)p.max_items + 2ll * gridDim.x;
+      long long works = 0;
+      for (int i = 0; i < kClasses; ++i) works += (long long)scratch->works[i] * p.kv_heads;
+      const int most = works > 0x7fffffff ? 0 : p.max_items + 2 * (int)gridDim.x;
       for (int k = 0;; ++k) {
         const int slot = k % kSlots;
         // An item is drawn only when its predecessor nears its end, so no CTA sits on work that
@@ -433,13 +460,13 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           break;
         }
         if (k > 0) {
-          if (lane == 0) w = (long long)gridDim.x + atomicAdd(counters + kTileNext, 1);
+          if (lane == 0) w = (int)gridDim.x + atomicAdd(counters + kTileNext, 1);
           w = __shfl_sync(0xffffffffu, w, 0);
         }
         while (c + 1 < kClasses && w >= class_end) {
-          class_end += (long long)scratch->works[++c] * p.kv_heads;
+          class_end += (int)scratch->works[++c] * p.kv_heads;
           b = p.batch;
-          before = (long long)scratch->works[c];
+          before = (int)scratch->works[c];
         }
         const bool more = w < class_end && w < most;
         Item it{};
@@ -450,15 +477,15 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
             const AttnRequest r = request_of(p, at);
             return class_of(p, r, share) == c ? pairs_of(p, r) * (c == 0 ? parts_of(r, share) : 1) : 0;
           };
-          const long long place = class_end - 1 - w, unit = place / p.kv_heads;
+          const int place = class_end - 1 - w, unit = (int)((unsigned)place / (unsigned)p.kv_heads);
           // Back over the requests, 32 at a time, to the one that holds `unit`.
           while (unit < before) {
             const int mine = b - 1 - lane;
             const int own = mine >= 0 ? units(mine) : 0;
-            long long upto = own;
-#pragma unroll
+            int upto = own;
+#pragma unroll 1
             for (int off = 1; off < 32; off <<= 1) {
-              const long long x = __shfl_up_sync(0xffffffffu, upto, off);
+              const int x = __shfl_up_sync(0xffffffffu, upto, off);
               if (lane >= off) upto += x;
             }
             const uint32_t reached = __ballot_sync(0xffffffffu, before - upto <= unit);
@@ -470,25 +497,29 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           // Inside a request: groups of key heads whose K and V stay in L2 while the group
           // runs, and in a group the last pairs (with the most keys) of all its heads first.
           const int pairs = pairs_of(p, r), parts = c == 0 ? parts_of(r, share) : 1;
-          const long long turn = (before + (long long)pairs * parts) * p.kv_heads - 1 - place;
-          const int heads_at_once = (int)min((long long)p.kv_heads, max(1ll, kGroupBytes / (4ll * HD * max(r.lk, 1))));
-          const long long in_group = (long long)heads_at_once * pairs * parts;
-          const int first_head = (int)(turn / in_group) * heads_at_once;
-          const int rest = (int)(turn % in_group), heads = min(heads_at_once, p.kv_heads - first_head);
-          const int tok0 = (pairs - 1 - rest / (heads * parts)) * 2 * p.tile_tokens;
-          const int part = rest % (heads * parts) / heads;
+          const int turn = (before + pairs * parts) * p.kv_heads - 1 - place;
+          const int heads_at_once =
+              min(p.kv_heads, max(1, (int)((unsigned)(kGroupBytes / (4 * HD)) / (unsigned)max(r.lk, 1))));
+          const int in_group = heads_at_once * pairs * parts;
+          const int groups_before = (int)((unsigned)turn / (unsigned)in_group);
+          const int first_head = groups_before * heads_at_once;
+          const int rest = turn - groups_before * in_group, heads = min(heads_at_once, p.kv_heads - first_head);
+          const int pair = (int)((unsigned)rest / (unsigned)(heads * parts)), at = rest - pair * heads * parts;
+          const int tok0 = (pairs - 1 - pair) * 2 * p.tile_tokens;
+          const int part = (int)((unsigned)at / (unsigned)heads);
           const bool has_b = tok0 + p.tile_tokens < r.lq;
           // Key tiles that each tile needs (of its last row), and this part's range of them.
           const int end_a = (visible_keys(p, r, min(tok0 + p.tile_tokens, r.lq) - 1) + BN - 1) / BN;
           const int end_b =
               has_b ? (visible_keys(p, r, min(tok0 + 2 * p.tile_tokens, r.lq) - 1) + BN - 1) / BN : 0;
           const int all = max(end_a, end_b);
-          const int lo = (int)((long long)part * all / parts), hi = (int)((long long)(part + 1) * all / parts);
+          const int lo = (int)((unsigned)(part * all) / (unsigned)parts);
+          const int hi = (int)((unsigned)((part + 1) * all) / (unsigned)parts);
           it.n = hi - lo;
           it.n_a = max(0, min(hi, end_a) - lo);
           it.n_b = max(0, min(hi, end_b) - lo);
           it.lo = lo;
-          it.hk = first_head + rest % (heads * parts) % heads;
+          it.hk = first_head + at - part * heads;
           it.b = b;
           it.row = r.q0 + tok0;
           it.valid = r.lq - tok0;
@@ -498,7 +529,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           it.last_rows = it.n > 0 && hi == r.lk / BN + 1 ? r.lk % BN : 0;
           it.parts = parts;
           it.part = part;
-          it.slot = c == 0 ? (int)(w - (long long)part * heads) : 0;
+          it.slot = c == 0 ? w - part * heads : 0;
           it.stride = heads;
         }
         if (lane == 0) {
@@ -617,9 +648,13 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           }
         }
         __syncwarp();
-        if (has_k) load(OFF_K + st * S::kTileBytes, &tmap_k, &bars->kv_full[st], cur.hk, row_of(cur, cur.lo + j), w_now);
-        if (has_v)
-          load(OFF_V + st * S::kTileBytes, &tmap_v, raw ? &bars->v_raw[st] : &bars->kv_full[st], v_hk, v_row, v_page);
+        const int k_row = row_of(cur, cur.lo + j);
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          if (!(t ? has_v : has_k)) continue;
+          load((t ? OFF_V : OFF_K) + st * S::kTileBytes, t ? &tmap_v : &tmap_k,
+               t && raw ? &bars->v_raw[st] : &bars->kv_full[st], t ? v_hk : cur.hk, t ? v_row : k_row, t ? v_page : w_now);
+        }
         ++kv_issued[st];
         ++step;
         has_v = has_k;
@@ -686,7 +721,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
             const uint32_t s_tmem = tmem + x * BN, o_tmem = tmem + (2 + x) * BN;
             if (pj < pnx) {
               const uint32_t parity = ((parities >> x) & 1) ^ 1;  // of the scores before
-#pragma unroll
+#pragma unroll 1
               for (int half = 0; half < 2; ++half) {
                 if (!mbar_wait(half ? &bars->p_full[x] : &bars->p_half[x], parity)) failed = 3;
                 tc_fence_after_sync();
@@ -820,26 +855,29 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       if (it->parts == 1) {
         reader.done(bars);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        uint32_t o[HD];
-        if (nx > 0) {
+        T* to = reinterpret_cast<T*>(p.o) + (first + i) * p.o_tok + (head0 + head) * p.o_head;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          if (nx > 0) {
+            tmem_ld_x32(o_tmem + c, o);
+            tmem_ld_wait();
+            reg_fence(o);
+          } else {
 #pragma unroll
-          for (int c = 0; c < HD; c += 32) tmem_ld_x32(o_tmem + c, reinterpret_cast<uint32_t(&)[32]>(o[c]));
-          tmem_ld_wait();
-          reg_fence(o);
-        } else {
-#pragma unroll
-          for (int c = 0; c < HD; ++c) o[c] = 0u;
-        }
-        if (in) {
-          T* to = reinterpret_cast<T*>(p.o) + (first + i) * p.o_tok + (head0 + head) * p.o_head;
-#pragma unroll
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t w[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              w[q] = pack2<T>(__uint_as_float(o[c + 2 * q]) * inv, __uint_as_float(o[c + 2 * q + 1]) * inv);
-            store32(to + c, w, wide);
+            for (int q = 0; q < 32; ++q) o[q] = 0u;
           }
+          if (in) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 16) {
+              uint32_t w[8];
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                w[q] = pack2<T>(__uint_as_float(o[d + 2 * q]) * inv, __uint_as_float(o[d + 2 * q + 1]) * inv);
+              store32(to + c + d, w, wide);
+            }
+          }
+          __syncwarp();
         }
         continue;
       }
