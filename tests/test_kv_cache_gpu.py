@@ -397,3 +397,51 @@ def test_an_invalid_capture_leaves_the_stream_usable(session):
         session.capture_end(rt.stream)
     b.enqueue()
     np.testing.assert_array_equal(b.outputs[0].to_numpy(rt.stream), want)
+
+
+def test_workspaces_come_and_go_beside_a_capture(session):
+    """While one stream is captured, another's workspace grows (its old one is freed) and an older
+    graph of attention operators is released: the capture stays valid, and nothing is put into it."""
+    rt = tb.Runtime(session)
+    other = tb.Runtime(session)
+    batch, h, hk, d, page, n = 2, 8, 2, 128, 16, 5000
+    pages = -(-n // page)
+    cache = [upload(session, rt.stream, rows((batch * pages, page, hk, d), DType.BF16, 980 + i), DType.BF16)
+             for i in range(2)]
+    table = ints(session, rt, np.arange(batch * pages).reshape(batch, pages))
+    lens = ints(session, rt, [n, n - 700])
+
+    def bind(runtime, tokens):
+        q = upload(session, rt.stream, rows((batch * tokens, h, d), DType.BF16, 990 + tokens), DType.BF16)
+        cu = ints(session, rt, np.arange(batch + 1) * tokens)
+        request = tb.OpRequest("attention.paged", [q, *cache, table, lens, cu], [spec_of(q)],
+                               {"max_query_len": tokens})
+        return runtime.bind(request, tb.TensorHandle.allocate(session, DType.BF16, q.shape))
+
+    small, large, mine = bind(other, 1), bind(other, 40), bind(rt, 3)
+    reference = bind(rt, 40)
+    for b in (small, mine, reference):  # (and their modules are loaded before the capture)
+        b.enqueue()
+    session.synchronize(rt.stream)
+    session.synchronize(other.stream)
+    want, want_large = (b.outputs[0].to_numpy(rt.stream) for b in (mine, reference))
+    session.capture_begin(rt.stream)
+    mine.enqueue()
+    old = session.capture_end(rt.stream)
+    old.launch(rt.stream)
+    session.synchronize(rt.stream)
+
+    session.capture_begin(rt.stream)
+    mine.enqueue()
+    with pytest.raises(tb.HalError, match="into a capture"):
+        old.launch(rt.stream)
+    large.enqueue()
+    old.release()
+    graph = session.capture_end(rt.stream)
+    session.synchronize(other.stream)
+    session.wait(session.upload(rt.stream, mine.outputs[0].buffer, np.zeros(want.shape, np.uint16)))
+    graph.launch(rt.stream)
+    session.synchronize(rt.stream)
+    np.testing.assert_array_equal(mine.outputs[0].to_numpy(rt.stream), want)
+    np.testing.assert_array_equal(large.outputs[0].to_numpy(other.stream), want_large)
+    graph.release()

@@ -11,7 +11,8 @@
 // host side runs at enqueue time), waits on the host, and an operator's first use of
 // per-stream scratch memory (it allocates), so such an operator runs once before capture.
 // The attention operators' workspace is the graph's own (stream_workspace): allocated at
-// capture, freed with the graph, shared with no other graph and no eager call.
+// capture, freed with the graph, shared with no other graph and no eager call. Graphs and
+// workspaces released while a stream is being captured are freed when the last capture ends.
 // A replay reads and writes the same device buffers the captured work named.
 #include "internal.hpp"
 
@@ -22,6 +23,8 @@ struct GraphExec : RefCounted {
   CUgraphExec exec = nullptr;
   std::vector<CUdeviceptr> work;  // workspace of its operators (stream_workspace)
   std::atomic<uint64_t> work_epoch{0};
+  CUevent done = nullptr;  // of its last launch, where it has workspace
+  std::mutex launch;       // keeps `done` in the launches' order
 };
 
 }  // namespace tb
@@ -40,6 +43,7 @@ tb_status tb_capture_begin(tb_session* session, tb_stream* stream) {
   if (rc) return rc;
   TB_CU("cuStreamBeginCapture", driver()->cuStreamBeginCapture_v2(st->raw, CU_STREAM_CAPTURE_MODE_THREAD_LOCAL));
   st->capture = capture_id(st);
+  if (st->capture) capture_began(s);
   return TB_OK;
 }
 
@@ -58,11 +62,12 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
   st->capture = 0;
   std::vector<CUdeviceptr> work = id ? take_captured_work(s, id) : std::vector<CUdeviceptr>();
   const auto drop_work = [&] {
-    for (CUdeviceptr p : work) d->cuMemFree_v2(p);
+    retire_work(s, {nullptr, work, nullptr});
   };
   // Ends the capture in every case; an invalidated capture (a call that cannot be
   // captured ran meanwhile) reports the driver's error and yields no graph.
   const CUresult ended = d->cuStreamEndCapture(st->raw, &graph);
+  if (id) capture_ended(s);
   if (ended != CUDA_SUCCESS || !graph) drop_work();
   if (ended != CUDA_SUCCESS) return cu_error("cuStreamEndCapture", ended);
   if (!graph) return set_error(TB_ERR_INVALID, "capture", "nothing was captured");
@@ -73,8 +78,18 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
     drop_work();
     return cu_error("cuGraphInstantiate", r);
   }
+  CUevent done = nullptr;
+  if (!work.empty()) {
+    const CUresult e = d->cuEventCreate(&done, CU_EVENT_DISABLE_TIMING);
+    if (e != CUDA_SUCCESS) {
+      d->cuGraphExecDestroy(exec);
+      drop_work();
+      return cu_error("cuEventCreate", e);
+    }
+  }
   GraphExec* g = new GraphExec();
   g->session = s;
+  g->done = done;
   g->exec = exec;
   g->work = std::move(work);
   g->work_epoch = s->work_epoch.load();
@@ -93,10 +108,20 @@ tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_str
   if (rc) return rc;
   rc = activate(s);
   if (rc) return rc;
-  if (const uint64_t epoch = s->work_epoch.load(); !g->work.empty() && g->work_epoch.exchange(epoch) != epoch)
+  const DriverApi* d = driver();
+  if (g->work.empty()) {
+    TB_CU("cuGraphLaunch", d->cuGraphLaunch(g->exec, st->raw));
+    return TB_OK;
+  }
+  // (A graph that took this one in would outlive its workspace.)
+  if (stream_capturing(st))
+    return set_error(TB_ERR_INVALID, "launch", "a graph with operators' workspace cannot be launched into a capture");
+  std::lock_guard<std::mutex> lock(g->launch);
+  if (const uint64_t epoch = s->work_epoch.load(); g->work_epoch.exchange(epoch) != epoch)
     for (CUdeviceptr p : g->work)
       if ((rc = clear_counters(st, p))) return rc;
-  TB_CU("cuGraphLaunch", driver()->cuGraphLaunch(g->exec, st->raw));
+  TB_CU("cuGraphLaunch", d->cuGraphLaunch(g->exec, st->raw));
+  TB_CU("cuEventRecord", d->cuEventRecord(g->done, st->raw));
   return TB_OK;
 }
 
@@ -107,9 +132,7 @@ void tb_graph_exec_release(tb_graph_exec* graph) {
   const DriverApi* d = driver();
   if (d && g->exec) {
     d->cuCtxSetCurrent(s->context);
-    d->cuGraphExecDestroy(g->exec);  // a replay still in flight completes; the driver frees it then
-    if (!g->work.empty()) d->cuCtxSynchronize();  // and may still use its workspace
-    for (CUdeviceptr p : g->work) d->cuMemFree_v2(p);
+    retire_work(s, {g->exec, g->work, g->done});
   }
   delete g;
   tb_session_release(reinterpret_cast<tb_session*>(s));

@@ -71,6 +71,13 @@ struct CapturedWork {
   size_t bytes;
 };
 
+// A graph (or none) and workspaces that are free once `last` has passed (none: at once).
+struct RetiredWork {
+  CUgraphExec exec;
+  std::vector<CUdeviceptr> work;
+  CUevent last;
+};
+
 struct Event : RefCounted {
   Session* session = nullptr;
   CUevent raw = nullptr;
@@ -115,6 +122,8 @@ struct Session : RefCounted {
   std::unordered_map<CUfunction, int> pair_occupancy;  // resident CTA pairs of a built-in pair kernel
   std::unordered_set<void*> pinned;
   std::vector<CapturedWork> captured_work;  // of captures that have not ended
+  std::vector<RetiredWork> retired;  // to be freed when no stream is being captured any more
+  int captures = 0;                  // streams being captured
   // Raised when a kernel reports that it gave up a wait: its workspace's counters may not be zero.
   std::atomic<uint64_t> work_epoch{0};
   StatusWord status;
@@ -141,6 +150,11 @@ tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* ou
 tb_status clear_counters(Stream* st, CUdeviceptr work);
 // The id of the capture that `st` is part of, 0 outside a capture.
 unsigned long long capture_id(Stream* st);
+// Frees a graph and workspaces when the work before `last` has ended: now, or, while a stream of
+// the session is being captured (which either would invalidate), when the last capture ends.
+void retire_work(Session* s, const RetiredWork& r);
+void capture_began(Session* s);
+void capture_ended(Session* s);
 // Takes the workspaces of an ended capture out of the session's list.
 std::vector<CUdeviceptr> take_captured_work(Session* s, unsigned long long capture);
 

@@ -189,6 +189,12 @@ void session_destroy(Session* s) {
   }
   for (const CapturedWork& w : s->captured_work)
     if (d) d->cuMemFree_v2(w.ptr);
+  for (const RetiredWork& r : s->retired) {
+    if (!d) break;
+    if (r.exec) d->cuGraphExecDestroy(r.exec);  // (every stream has been waited for)
+    if (r.last) d->cuEventDestroy_v2(r.last);
+    for (CUdeviceptr p : r.work) d->cuMemFree_v2(p);
+  }
   for (void* p : s->pinned)
     if (d) d->cuMemFreeHost(p);
   if (d && s->status.host) d->cuMemFreeHost((void*)s->status.host);
@@ -306,6 +312,45 @@ unsigned long long capture_id(Stream* st) {
   return id;
 }
 
+namespace {
+
+void free_work(const RetiredWork& r) {
+  const DriverApi* d = driver();
+  if (r.exec) d->cuGraphExecDestroy(r.exec);  // a replay still in flight completes; the driver frees it then
+  if (r.last) {
+    d->cuEventSynchronize(r.last);
+    d->cuEventDestroy_v2(r.last);
+  }
+  for (CUdeviceptr p : r.work) d->cuMemFree_v2(p);
+}
+
+}  // namespace
+
+void retire_work(Session* s, const RetiredWork& r) {
+  {
+    std::lock_guard<std::mutex> lock(s->mu);
+    if (s->captures > 0) {
+      s->retired.push_back(r);
+      return;
+    }
+  }
+  free_work(r);
+}
+
+void capture_began(Session* s) {
+  std::lock_guard<std::mutex> lock(s->mu);
+  ++s->captures;
+}
+
+void capture_ended(Session* s) {
+  std::vector<RetiredWork> free_now;
+  {
+    std::lock_guard<std::mutex> lock(s->mu);
+    if (--s->captures == 0) free_now.swap(s->retired);
+  }
+  for (const RetiredWork& r : free_now) free_work(r);
+}
+
 std::vector<CUdeviceptr> take_captured_work(Session* s, unsigned long long capture) {
   std::vector<CUdeviceptr> got;
   std::lock_guard<std::mutex> lock(s->mu);
@@ -367,8 +412,13 @@ tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* ou
     const DriverApi* d = driver();
     if (st->work) {
       // Earlier kernels on this stream may still use the old one.
-      TB_CU("cuStreamSynchronize", d->cuStreamSynchronize(st->raw));
-      d->cuMemFree_v2(st->work);
+      CUevent last = nullptr;
+      TB_CU("cuEventCreate", d->cuEventCreate(&last, CU_EVENT_DISABLE_TIMING));
+      if (const CUresult r = d->cuEventRecord(last, st->raw); r != CUDA_SUCCESS) {
+        d->cuEventDestroy_v2(last);
+        return cu_error("cuEventRecord", r);
+      }
+      retire_work(s, {nullptr, {st->work}, last});
       st->work = 0;
       st->work_bytes = 0;
     }
@@ -611,9 +661,13 @@ void tb_stream_release(tb_stream* stream) {
     if (x->scratch || x->work) {
       d->cuStreamSynchronize(x->raw);
       if (x->scratch) d->cuMemFree_v2(x->scratch);
-      if (x->work) d->cuMemFree_v2(x->work);
+      if (x->work) retire_work(s, {nullptr, {x->work}, nullptr});
     }
     d->cuStreamDestroy_v2(x->raw);
+    if (x->capture) {  // a capture that nothing ends any more
+      retire_work(s, {nullptr, take_captured_work(s, x->capture), nullptr});
+      capture_ended(s);
+    }
   }
   delete x;
   session_unref(s);
