@@ -219,10 +219,10 @@ tb_status run_attention(Session* s, Stream* st, const char* op, AttnCall* c, con
     return unsupported("candidate " + only + " does not take this shape, page size, alignment or max_query_len");
   std::lock_guard<std::mutex> lock(st->enqueue);
   // Steps of few rows are the token kernel's. Other steps take one launch of the tile kernel for
-  // all requests: it reads single tokens' keys more slowly (64 requests of 300-8192 keys 128 us
-  // against 97, four of 110-131 thousand 600 against 304), but a launch of each kernel costs
-  // more where chunks fill the step (eight requests, two of them single tokens, 150 us
-  // against 124). Where tiles do not fit, the token kernel still takes the single tokens.
+  // all requests: it reads single tokens' keys more slowly (64 requests of 300-8192 keys 119 us
+  // against 97, four of 110-131 thousand 575 against 305), but a launch of each kernel costs
+  // more where chunks fill the step (eight requests, two of them single tokens, 136 us
+  // against 121). Where tiles do not fit, the token kernel still takes the single tokens.
   if (few || (tokens && !tiles && group <= 32)) {
     const uint64_t rows = few ? longest * group : group;
     c->p.token_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
