@@ -1,0 +1,53 @@
+"""The library's host side on a stand-in driver: what threads, sizes and requests make of a
+stream's memory and a kernel's limits."""
+import pytest
+
+import host_driver
+
+pytestmark = host_driver.needs_compiler
+
+
+@pytest.fixture(scope="module")
+def driver(tmp_path_factory):
+    return host_driver.build_driver(tmp_path_factory.mktemp("driver"))
+
+
+SCRATCH_USERS = """
+def gemm(m, n, k, **attrs):
+    a, b = (tb.TensorHandle.allocate(session, DType.BF16, s) for s in ((m, k), (n, k)))
+    c = tb.TensorHandle.allocate(session, DType.BF16, (m, n))
+    return rt.bind(tb.OpRequest("gemm", [a, b], [spec_of(c)], {"transpose_rhs": True, **attrs}), c)
+
+def sdpa(t):
+    x = tb.TensorHandle.allocate(session, DType.BF16, (1, 1, t, 128))
+    return rt.bind(tb.OpRequest("scaled_dot_product_attention", [x] * 3, [spec_of(x)],
+                                {"candidate": "sdpa_fwd_bf16_d128_persist"}), x)
+
+def hammer(*requests):
+    fake.fake_slow(3)
+    in_threads(*[lambda r=r: [r.enqueue() for _ in range(8)] for r in requests])
+    fake.fake_slow(0)
+    seen = lines()
+    assert not [x for x in seen if x.startswith("error")], [x for x in seen if x.startswith("error")]
+    return [x.split()[1:] for x in seen]
+"""
+
+
+def test_threads_share_a_stream_s_scratch(driver):
+    """Requests of several threads on one stream, of operators that take its scratch memory: none is
+    launched on memory that a larger one replaced, and none comes between another's kernels."""
+    host_driver.run(driver, SCRATCH_USERS + """
+small, large = gemm(128, 128, 4096), gemm(256, 512, 4096)
+launches = hammer(small, large)
+assert {x[0] for x in launches} == {"gemm_bf16_tn_splitk", "splitk_reduce_bf16"}
+for first, second in zip(launches[::2], launches[1::2]):
+    assert first[0] == "gemm_bf16_tn_splitk" and second[0] == "splitk_reduce_bf16" and first[1:] == second[1:]
+
+rt = tb.Runtime(session)
+launches = hammer(gemm(512, 512, 513), gemm(1024, 1024, 513), sdpa(300))
+names = [x[0] for x in launches]
+for i, name in enumerate(names):  # two staged operands, then their product
+    if name == "stage_bf16_pad_rows":
+        if names[i - 1] != name:
+            assert names[i + 1] == name and names[i + 2].startswith("gemm_bf16_tn"), names[i:i + 4]
+""")

@@ -50,6 +50,7 @@ struct Stream : RefCounted {
   CUstream raw = nullptr;
   // Scratch device memory for kernels launched on this stream (split-K partials).
   // Stream order serialises its users; it grows on demand and is freed with the stream.
+  // As the workspace below, it is taken and its kernels launched with `enqueue` held.
   CUdeviceptr scratch = 0;
   size_t scratch_bytes = 0;
   // Workspace of the attention operators (zeroed when allocated, and left with its counters
@@ -140,7 +141,8 @@ tb_status check_buffer(Session* s, tb_buffer* b, Buffer** out);
 tb_status check_stream(Session* s, tb_stream* st, Stream** out);
 tb_status check_event(Session* s, tb_event* e, Event** out);
 
-// At least `bytes` of the stream's scratch memory (allocating or growing it).
+// At least `bytes` of the stream's scratch memory (allocating or growing it). The caller holds
+// st->enqueue until it has launched the last kernel that uses it.
 tb_status stream_scratch(Session* s, Stream* st, size_t bytes, CUdeviceptr* out);
 
 // At least `bytes` of zeroed-at-first workspace for an operator on the stream: the stream's

@@ -181,6 +181,7 @@ static tb_status launch_gemm_bf16_staged(Session* s, Stream* st, CUdeviceptr a, 
   const size_t c_span = stage_c ? (size_t)M * c_pitch * 2 : 0;
   CUdeviceptr ws = 0;
   tb_status rc = TB_OK;
+  std::lock_guard<std::mutex> lock(st->enqueue);  // of the scratch, until its last reader is launched
   if (a_span + b_span + c_span) rc = stream_scratch(s, st, a_span + b_span + c_span, &ws);
   if (rc) return rc;
   const CUdeviceptr ka = stage_a ? ws : a, kb = stage_b ? ws + a_span : b, kc = stage_c ? ws + a_span + b_span : c;
@@ -445,6 +446,7 @@ extern "C" tb_status tb_op_gemm(tb_session* session, tb_stream* stream, const tb
     if (force_split && plan.splits < 2) return unsupported("candidate gemm_bf16_tn_splitk needs at least 2 k-blocks");
     if (tma_ok && !want_generic && plan.splits >= 2) {
       CUdeviceptr partial = 0;
+      std::lock_guard<std::mutex> lock(st->enqueue);  // of the scratch, until its last reader is launched
       rc = stream_scratch(s, st, (size_t)plan.splits * M * N * sizeof(float), &partial);
       if (rc) return rc;
       rc = launch_gemm_bf16_splitk(s, st, pa, pb, pc, M, N, K, (long long)N, plan.splits, plan.kb_per_split,

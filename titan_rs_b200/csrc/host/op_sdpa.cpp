@@ -102,6 +102,7 @@ tb_status launch_sdpa_bf16_d128_persist(Session* s, Stream* st, CUdeviceptr q, C
   const unsigned grid = (unsigned)std::min<unsigned long long>(items, (unsigned long long)s->sm_count);
   // The work-item counter the CTAs draw from, zeroed in stream order before the launch.
   CUdeviceptr next_item = 0;
+  std::lock_guard<std::mutex> lock(st->enqueue);  // of the scratch, until its reader is launched
   if ((rc = stream_scratch(s, st, sizeof(uint32_t), &next_item))) return rc;
   TB_CU("cuMemsetD32Async", driver()->cuMemsetD32Async(next_item, 0, 1, st->raw));
   void* params[] = {&mq, &mk, &mv, &o, &bh, &tq, &tk, &causal, &scale_log2, &next_item, &status};
