@@ -51,3 +51,25 @@ for i, name in enumerate(names):  # two staged operands, then their product
         if names[i - 1] != name:
             assert names[i + 1] == name and names[i + 2].startswith("gemm_bf16_tn"), names[i:i + 4]
 """)
+
+
+def test_every_plan_has_its_shared_memory(driver):
+    """kv_cache.plan's dynamic shared memory grows with the batch, beside static bytes: around 48 KB
+    together, and from threads whose batches differ."""
+    host_driver.run(driver, """
+def plan(runtime, batch):
+    ints = lambda *shape: tb.TensorHandle.allocate(session, DType.I32, shape)
+    outs = [ints(batch, 2), ints(batch), ints(batch + 1), ints(batch), ints(2)]
+    return runtime.bind(tb.OpRequest("kv_cache.plan", [ints(batch), ints(batch), ints(4)],
+                                     [spec_of(t) for t in outs], {"page_size": 16}), outs)
+
+for batch in (6109, 6110, 6143, 6144, 16384, 6120):
+    plan(rt, batch).enqueue()
+fake.fake_slow(2)
+requests = [plan(tb.Runtime(session), batch) for batch in (6500, 9000, 12000, 16000)]
+in_threads(*[lambda r=r: [r.enqueue() for _ in range(20)] for r in requests])
+session.close()
+session = tb.Session(0)  # (a fresh limit)
+requests = [plan(tb.Runtime(session), batch) for batch in (6500, 9000, 12000, 16000)]
+in_threads(*[lambda r=r: [r.enqueue() for _ in range(20)] for r in requests])
+""")

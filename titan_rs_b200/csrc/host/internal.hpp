@@ -121,6 +121,7 @@ struct Session : RefCounted {
   std::unordered_map<std::string, CUfunction> builtin_functions;        // embedded cubin entries
   std::unordered_map<std::string, std::shared_ptr<Module>> builtin_modules;
   std::unordered_map<CUfunction, int> pair_occupancy;  // resident CTA pairs of a built-in pair kernel
+  std::unordered_map<CUfunction, int> shared_limit;  // dynamic shared memory that a kernel may be launched with
   std::unordered_set<void*> pinned;
   std::vector<CapturedWork> captured_work;  // of captures that have not ended
   std::vector<RetiredWork> retired;  // to be freed when no stream is being captured any more

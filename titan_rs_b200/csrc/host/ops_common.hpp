@@ -168,14 +168,33 @@ inline tb_status launch_builtin(Session* s, Stream* st, CUfunction fn, unsigned 
   return TB_OK;
 }
 
+// Raises a built-in kernel's limit of dynamic shared memory to `bytes` where it is lower. It
+// starts at 48 KB less the kernel's static bytes, and is never lowered, so that launches of
+// several sizes from several threads do not take it from each other.
+inline tb_status allow_shared(Session* s, CUfunction fn, unsigned bytes) {
+  if (bytes <= 16 * 1024) return TB_OK;  // (no kernel here has 32 KB of static bytes)
+  const DriverApi* d = driver();
+  std::lock_guard<std::mutex> lock(s->mu);
+  auto it = s->shared_limit.find(fn);
+  if (it == s->shared_limit.end()) {
+    int fixed = 0;
+    TB_CU("cuFuncGetAttribute", d->cuFuncGetAttribute(&fixed, CU_FUNC_ATTRIBUTE_SHARED_SIZE_BYTES, fn));
+    it = s->shared_limit.emplace(fn, 48 * 1024 - fixed).first;
+  }
+  if ((int)bytes > it->second) {
+    TB_CU("cuFuncSetAttribute",
+          d->cuFuncSetAttribute(fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)bytes));
+    it->second = (int)bytes;
+  }
+  return TB_OK;
+}
+
 // Launches a built-in kernel that begins by waiting for the grids before it
 // (griddepcontrol.wait), so that its blocks may be set up while those still run.
 inline tb_status launch_overlapped(Session* s, Stream* st, CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
                                    unsigned shared_bytes, void** params, const char* candidate) {
   const DriverApi* d = driver();
-  if (shared_bytes > 48 * 1024)
-    TB_CU("cuFuncSetAttribute",
-          d->cuFuncSetAttribute(fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)shared_bytes));
+  if (const tb_status rc = allow_shared(s, fn, shared_bytes)) return rc;
   CUlaunchConfig cfg{};
   cfg.gridDimX = gx;
   cfg.gridDimY = gy;
@@ -191,7 +210,6 @@ inline tb_status launch_overlapped(Session* s, Stream* st, CUfunction fn, unsign
   cfg.numAttrs = 1;
   TB_CU("cuLaunchKernelEx", d->cuLaunchKernelEx(&cfg, fn, params, nullptr));
   note_launch(candidate);
-  (void)s;
   return TB_OK;
 }
 
