@@ -34,3 +34,40 @@ def test_plan_of_every_batch_launches(session, rt):
         ctx, new, free, table = random_plan(rng, batch, 9, 2, 4)
         got = assert_plan(session, rt, ctx, new, free, table, int(new.sum()) + 1, 4)
         assert got[4][1] == 0
+
+
+def test_outputs_are_written_where_their_tensors_lie(session, rt):
+    """Specs without strides beside strided outputs: a cache with heads before rows, an attention
+    output inside a wider tensor, a block table with wider rows."""
+    hk, h, d, page, pages, t, dtype = 2, 4, 64, 8, 4, 5, DType.BF16
+    host = rows((t, hk, d), dtype, 1)
+    k = upload(session, rt.stream, host, dtype)
+    base = upload(session, rt.stream, np.zeros((2, pages, hk, page, d), np.uint16), dtype)
+    caches = [view(session, base, i * pages * hk * page * d, (pages, page, hk, d), (hk * page * d, d, page * d, 1))
+              for i in range(2)]
+    slots = [0, 9, 17, 3, 30]
+    rt.execute(tb.OpRequest("kv_cache.append", [k, k, ints(session, rt, slots)],
+                            [tb.TensorSpec(dtype, c.shape) for c in caches]), output=caches).wait()
+    want = np.zeros((2, pages, hk, page, d), np.uint16)
+    for n, slot in enumerate(slots):
+        want[:, slot // page, :, slot % page] = host[n]
+    np.testing.assert_array_equal(base.to_numpy(rt.stream), want)
+
+    q = upload(session, rt.stream, rows((t, h, d), dtype, 2), dtype)
+    wide = upload(session, rt.stream, np.zeros((t, h, d + 24), np.uint16), dtype)
+    o = view(session, wide, 0, (t, h, d), (h * (d + 24), d + 24, 1))
+    inputs = [q, k, k, ints(session, rt, [0, 2, 5])]
+    plain = rt.execute(tb.OpRequest("attention.varlen", inputs, [tb.TensorSpec(dtype, (t, h, d))])).wait()
+    got = rt.execute(tb.OpRequest("attention.varlen", inputs, [tb.TensorSpec(dtype, (t, h, d))]), output=o).wait()
+    assert got.outputs[0].strides == o.strides
+    after = wide.to_numpy(rt.stream)
+    np.testing.assert_array_equal(after[:, :, :d], plain.outputs[0].to_numpy(rt.stream))
+    np.testing.assert_array_equal(after[:, :, d:], 0)
+
+    table = ints(session, rt, np.full((2, 5), -3))
+    outs = [tb.TensorHandle(session, table.buffer, DType.I32, (2, 2), (5, 1)), ints(session, rt, [0, 0]),
+            ints(session, rt, [0, 0, 0]), ints(session, rt, [0] * 9), ints(session, rt, [0, 0])]
+    rt.bind(tb.OpRequest("kv_cache.plan", [ints(session, rt, x) for x in ([0, 0], [9, 3], [5, 6, 7])],
+                         [tb.TensorSpec(DType.I32, x.shape) for x in outs], {"page_size": 8}), outs).enqueue()
+    # (The second request's tokens, 9 to 11, pass the end of the slot map: it is refused.)
+    np.testing.assert_array_equal(table.to_numpy(rt.stream), [[5, 6, -3, -3, -3], [-3, -3, -3, -3, -3]])

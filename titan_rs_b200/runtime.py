@@ -182,6 +182,9 @@ _ARITY = {"softmax": (1, 1), "gemm": (2, 2), "scaled_dot_product_attention": (3,
 # Operators with several outputs. They write into tensors that already hold something (the
 # caches, the block table), so the caller passes these.
 _OUTPUTS = {"kv_cache.append": 2, "kv_cache.plan": 5}
+# Operators whose outputs may be strided. What the request says of such an output has to be what
+# the tensor passed for it is, since a wrong stride puts its rows elsewhere in the same memory.
+_STRIDED_OUTPUTS = {"attention.varlen", "attention.paged", "kv_cache.append", "kv_cache.plan"}
 _ARITY_MSG = {"softmax": "CUDA softmax requires exactly one input and one output",
               "gemm": "gemm requires exactly two rank-2 inputs",
               "scaled_dot_product_attention": "scaled dot-product attention requires exactly three rank-4 BHTD inputs",
@@ -215,9 +218,11 @@ class Runtime:
 
     def execute(self, request: OpRequest, output=None) -> ExecutionHandle:
         """Enqueues a request. `output`: the tensor to write, or the list of them for an operator
-        of several outputs; one output may be left out and is then allocated."""
+        of several outputs; one output may be left out and is then allocated. An operator whose
+        outputs may be strided takes the strides of the tensor where the request's spec names none,
+        and refuses a tensor that differs from its spec."""
         name = request.operator
-        outputs = self._checked(request, output)
+        request, outputs = self._checked(request, output)
         attrs = dict(request.attrs)
         self.last_tune = None
         if self.autotuner is not None and "candidate" not in attrs and len(outputs) == 1:
@@ -232,10 +237,10 @@ class Runtime:
     def bind(self, request: OpRequest, output=None) -> "BoundRequest":
         """A request that is enqueued many times over the same tensors (a serving step): its
         arguments cross the ABI once, and each BoundRequest.enqueue() is one native call."""
-        return BoundRequest(self, request, self._checked(request, output))
+        return BoundRequest(self, *self._checked(request, output))
 
-    def _checked(self, request: OpRequest, output) -> list:
-        """The request's checks on this side of the ABI, and its output tensors."""
+    def _checked(self, request: OpRequest, output) -> tuple:
+        """The request's checks on this side of the ABI; the request and its output tensors."""
         name = request.operator
         if name not in _OPS:
             raise ExecutionError(name, "contract", f"operator {name} is not on the B200 hot path (does not implement)",
@@ -249,14 +254,28 @@ class Runtime:
         if output is None and name not in _OUTPUTS:
             spec = request.outputs[0]
             try:
-                return [TensorHandle.allocate(self.session, spec.dtype, spec.shape)]
+                return request, [TensorHandle.allocate(self.session, spec.dtype, spec.shape)]
             except HalError as e:
                 raise ExecutionError(name, "allocate", str(e), e.status) from e
         outputs = list(output) if isinstance(output, (list, tuple)) else [] if output is None else [output]
         if len(outputs) != len(request.outputs):
             raise ExecutionError(name, "contract", f"{name} writes into existing tensors: pass "
                                                    f"output=[{len(request.outputs)} tensors]")
-        return outputs
+        if name in _STRIDED_OUTPUTS:
+            specs = [self._spec_of_output(name, *pair) for pair in zip(request.outputs, outputs)]
+            request = OpRequest(name, request.inputs, specs, request.attrs)
+        return request, outputs
+
+    @staticmethod
+    def _spec_of_output(name: str, spec: TensorSpec, tensor: TensorHandle) -> TensorSpec:
+        shape = tuple(spec.shape)
+        same = spec.dtype == tensor.dtype and shape == tuple(tensor.shape)
+        if same and spec.strides is not None and spec.layout == "Contiguous":  # (a stride of an extent of one is free)
+            same = all(n <= 1 or a == b for n, a, b in zip(shape, spec.strides, tensor.strides))
+        if not same:
+            raise ExecutionError(name, "contract", f"{name} requires output tensors of their specs' dtype, shape and "
+                                                   "strides")
+        return TensorSpec(spec.dtype, shape, tuple(tensor.strides), spec.layout)
 
     def _result(self, request: OpRequest, outputs: list) -> list:
         return [TensorHandle(self.session, t.buffer, spec.dtype, tuple(spec.shape),
