@@ -1,4 +1,8 @@
 """The serving operators' checks that need no GPU, beyond those of test_serving_cpu.py."""
+import pathlib
+import shutil
+import subprocess
+
 import pytest
 
 import titan_rs_b200 as tb
@@ -36,3 +40,41 @@ def test_an_output_has_to_be_its_spec(operator, dtype, shape):
                          (tb.TensorSpec(dtype, shape), handle(dtype, shape[1:]))]:
         with pytest.raises(tb.ExecutionError, match="their specs' dtype, shape and strides"):
             outputs(spec, tensor)
+
+
+BANKS = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+#include "attn_params.cuh"
+using namespace tb;
+int main() {
+  std::vector<int> work(kWorkFront / 4, 0);  // as a workspace begins
+  const int grids[] = {148, 3, 148, 1, 1, 148, 512, 2, 148, 148};
+  for (int n = 0; n < 200; ++n) {
+    const int grid = grids[n % 10], threads = grid * 32, turn = work[kTileTurn];
+    for (int slot = 0; slot < 2 * kTileMaxCtas; ++slot)
+      for (int x = 0; x < 2; ++x)
+        if (work[tile_parts_at(turn, slot, x)] != 0) return std::printf("launch %d, slot %d\n", n, slot), 1;
+    for (int id = 0; id < threads; ++id) clear_next_bank(work.data(), turn, id, threads);
+    // Finished parts of all of the launch's slots: whatever a wait that ran out leaves.
+    for (int slot = 0; slot < 2 * grid; ++slot)
+      for (int x = 0; x < 2; ++x) work[tile_parts_at(turn, slot, x)] = std::rand() % 33;
+    work[kTileTurn] = turn ^ 1;
+  }
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no C++ compiler on this machine")
+def test_no_launch_counts_parts_of_an_earlier_one(tmp_path):
+    """The counters of finished parts, as a row of launches of different grids uses and clears them:
+    each finds its own at zero, whatever the ones before left."""
+    kernels = pathlib.Path(__file__).resolve().parents[1] / "titan_rs_b200" / "csrc" / "kernels"
+    (tmp_path / "banks.cpp").write_text(BANKS)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined,address", "-I", str(kernels),
+                    str(tmp_path / "banks.cpp"), "-o", str(tmp_path / "banks")], check=True, capture_output=True,
+                   text=True)
+    done = subprocess.run([str(tmp_path / "banks")], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr

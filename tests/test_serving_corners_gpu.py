@@ -71,3 +71,31 @@ def test_outputs_are_written_where_their_tensors_lie(session, rt):
                          [tb.TensorSpec(DType.I32, x.shape) for x in outs], {"page_size": 8}), outs).enqueue()
     # (The second request's tokens, 9 to 11, pass the end of the slot map: it is refused.)
     np.testing.assert_array_equal(table.to_numpy(rt.stream), [[5, 6, -3, -3, -3], [-3, -3, -3, -3, -3]])
+
+
+def test_cut_requests_one_behind_another(session):
+    """Requests whose keys are cut into parts, of different sizes and grids, launched in turn on one
+    stream: every launch gives the same result."""
+    page, dtype, d = 16, DType.BF16, 64
+    runtime = tb.Runtime(session)
+    bound = []
+    for lens, new, h, hk in (([6000], [70], 4, 1), ([3000, 70, 1100], [20, 20, 20], 8, 2), ([700], [40], 2, 1)):
+        cu = prefix(new)
+        k, v, table = make_cache(lens, page, hk, d, dtype, 40 + h)
+        q = upload(session, runtime.stream, rows((int(cu[-1]), h, d), dtype, 50 + h), dtype)
+        ins = [q] + [upload(session, runtime.stream, x, dtype) for x in (k, v)]
+        ins += [ints(session, runtime, x) for x in (table, lens, cu)]
+        request = tb.OpRequest("attention.paged", ins, [spec_of(q)], {"candidate": "attention_tiles"})
+        bound.append(runtime.bind(request, tb.TensorHandle.allocate(session, dtype, q.shape)))
+    want = []
+    for b in bound:
+        b.enqueue()
+        want.append(b.outputs[0].to_numpy(runtime.stream))
+    for n in range(60):
+        bound[(n * n) % 3].enqueue()
+        bound[n % 3].enqueue()
+        if n % 7 == 0:
+            for b, w in zip(bound, want):
+                np.testing.assert_array_equal(b.outputs[0].to_numpy(runtime.stream), w)
+    for b, w in zip(bound, want):
+        np.testing.assert_array_equal(b.outputs[0].to_numpy(runtime.stream), w)

@@ -22,7 +22,6 @@ struct GraphExec : RefCounted {
   Session* session = nullptr;
   CUgraphExec exec = nullptr;
   std::vector<CUdeviceptr> work;  // workspace of its operators (stream_workspace)
-  std::atomic<uint64_t> work_epoch{0};
   CUevent done = nullptr;  // of its last launch, where it has workspace
   std::mutex launch;       // keeps `done` in the launches' order
 };
@@ -92,7 +91,6 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
   g->done = done;
   g->exec = exec;
   g->work = std::move(work);
-  g->work_epoch = s->work_epoch.load();
   s->refs.fetch_add(1);
   *out = reinterpret_cast<tb_graph_exec*>(g);
   return TB_OK;
@@ -117,9 +115,6 @@ tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_str
   if (stream_capturing(st))
     return set_error(TB_ERR_INVALID, "launch", "a graph with operators' workspace cannot be launched into a capture");
   std::lock_guard<std::mutex> lock(g->launch);
-  if (const uint64_t epoch = s->work_epoch.load(); g->work_epoch.exchange(epoch) != epoch)
-    for (CUdeviceptr p : g->work)
-      if ((rc = clear_counters(st, p))) return rc;
   TB_CU("cuGraphLaunch", d->cuGraphLaunch(g->exec, st->raw));
   TB_CU("cuEventRecord", d->cuEventRecord(g->done, st->raw));
   return TB_OK;

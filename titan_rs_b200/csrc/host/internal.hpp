@@ -53,12 +53,12 @@ struct Stream : RefCounted {
   // As the workspace below, it is taken and its kernels launched with `enqueue` held.
   CUdeviceptr scratch = 0;
   size_t scratch_bytes = 0;
-  // Workspace of the attention operators (zeroed when allocated, and left with its counters
-  // at zero by every launch). `enqueue` is held while an operator takes it and launches, so
-  // that a second host thread on the stream cannot replace it in between.
+  // Workspace of the attention operators (zeroed when allocated; every launch leaves its counters
+  // as the next one needs them, also one that gave up a wait). `enqueue` is held while an
+  // operator takes it and launches, so that a second host thread on the stream cannot replace it
+  // in between.
   CUdeviceptr work = 0;
   size_t work_bytes = 0;
-  uint64_t work_epoch = 0;  // Session::work_epoch when its counters were last known to be zero
   std::mutex enqueue;
   unsigned long long capture = 0;  // the driver's id of the capture that tb_capture_begin began
 };
@@ -126,8 +126,6 @@ struct Session : RefCounted {
   std::vector<CapturedWork> captured_work;  // of captures that have not ended
   std::vector<RetiredWork> retired;  // to be freed when no stream is being captured any more
   int captures = 0;                  // streams being captured
-  // Raised when a kernel reports that it gave up a wait: its workspace's counters may not be zero.
-  std::atomic<uint64_t> work_epoch{0};
   StatusWord status;
   int sm_count = 0;
   int max_smem_optin = 0;
@@ -149,8 +147,6 @@ tb_status stream_scratch(Session* s, Stream* st, size_t bytes, CUdeviceptr* out)
 // At least `bytes` of zeroed-at-first workspace for an operator on the stream: the stream's
 // own, or, while the stream is being captured, memory of the graph. The caller holds st->enqueue.
 tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* out);
-// Zeroes the counters at a workspace's front, in stream order.
-tb_status clear_counters(Stream* st, CUdeviceptr work);
 // The id of the capture that `st` is part of, 0 outside a capture.
 unsigned long long capture_id(Stream* st);
 // Frees a graph and workspaces when the work before `last` has ended: now, or, while a stream of

@@ -13,7 +13,6 @@
 #include <cstdio>
 #include <cstdlib>
 
-#include "../kernels/attn_params.cuh"
 #include "internal.hpp"
 
 namespace tb {
@@ -151,7 +150,6 @@ tb_status consume_device_status(Session* s) {
   uint32_t code = *s->status.host;
   if (code == 0) return TB_OK;
   *s->status.host = 0;
-  s->work_epoch.fetch_add(1);
   char buf[160];
   snprintf(buf, sizeof buf,
            "a kernel gave up a bounded device-side wait (code 0x%08x); its output is invalid, the context is usable",
@@ -387,11 +385,6 @@ tb_status zeroed_memory(size_t bytes, CUdeviceptr* out) {
 
 }  // namespace
 
-tb_status clear_counters(Stream* st, CUdeviceptr work) {
-  TB_CU("cuMemsetD8Async", driver()->cuMemsetD8Async(work, 0, kWorkFront, st->raw));
-  return TB_OK;
-}
-
 tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* out) {
   if (const unsigned long long id = capture_id(st)) {
     {
@@ -425,12 +418,6 @@ tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* ou
     tb_status rc = zeroed_memory(bytes, &st->work);
     if (rc) return rc;
     st->work_bytes = bytes;
-    st->work_epoch = s->work_epoch.load();
-  }
-  if (const uint64_t epoch = s->work_epoch.load(); st->work_epoch != epoch) {
-    tb_status rc = clear_counters(st, st->work);
-    if (rc) return rc;
-    st->work_epoch = epoch;
   }
   *out = st->work;
   return TB_OK;

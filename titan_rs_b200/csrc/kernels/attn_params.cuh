@@ -41,13 +41,22 @@ struct AttnParams {
                            // workspace then has two slots for each CTA)
 };
 
-// The front of every workspace holds counters that are zero between launches, at the same
-// place for every kernel and form: one per CTA of the token kernel; the tile kernel's next
-// work number and its count of finished CTAs; and the finished parts of each of its slots' two
-// tiles.
-constexpr int kTokenMaxCtas = 1022, kTileNext = 1022, kTileDone = 1023, kTileParts = 1024;
+// The front of every workspace holds counters, at the same place for every kernel and form. Zero
+// between launches are one per CTA of the token kernel, and the tile kernel's next work number
+// and its count of finished CTAs: nothing keeps a kernel from bringing them back. The finished
+// parts of each of the tile kernel's slots' two tiles stay behind, since a launch that gave up a
+// wait may leave any of them at any value. They are held twice: launches that cut items use
+// the two banks in turn (kTileTurn says which) and clear the other bank for the next one, so that
+// none sees what an earlier one left.
+constexpr int kTokenMaxCtas = 1022, kTileNext = 1022, kTileDone = 1023, kTileTurn = 1024, kTileParts = 1056;
 constexpr int kTileMaxCtas = 512;
-constexpr uint64_t kWorkFront = 4ull * (kTileParts + 2 * 2 * kTileMaxCtas);
+constexpr int kTileBank = 2 * 2 * kTileMaxCtas;
+constexpr uint64_t kWorkFront = 4ull * (kTileParts + 2 * kTileBank);
+// (Workspace offsets of both kernels are multiples of their widest store, 32 bytes.)
+static_assert(kWorkFront % 128 == 0 && kTileParts % 32 == 0 && kTileBank % 4 == 0, "workspace alignment");
+TB_BOTH constexpr int tile_bank(int turn) { return kTileParts + turn * kTileBank; }
+// The counter of finished parts of a slot's tile x (0 or 1).
+TB_BOTH constexpr int tile_parts_at(int turn, int slot, int x) { return tile_bank(turn) + 2 * slot + x; }
 
 // The token kernel's partial results, behind the counters: two a CTA (its first request may
 // have begun in an earlier CTA, its last may go on in a later one), each rows x (dim + 2)
@@ -131,6 +140,13 @@ TB_INDEX_FN AttnRequest request_of(const AttnParams& p, int b) {
     r.lk = clamp_index(load_index(cu_k + b + 1), r.k0, p.tk) - r.k0;
   }
   return r;
+}
+
+// Clears the counters that the next launch counts finished parts in: thread `id` of `threads`
+// over the whole grid takes every `threads`-th four of them.
+TB_INDEX_FN void clear_next_bank(int* counters, int turn, int id, int threads) {
+  for (int i = id; i < kTileBank / 4; i += threads)
+    for (int k = 0; k < 4; ++k) counters[tile_bank(turn ^ 1) + 4 * i + k] = 0;
 }
 
 // Whether the request is the token kernel's (it has query rows, and few enough).

@@ -412,6 +412,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
     tmem_relinquish();
   }
   begin_after_earlier_grids();
+  const int turn = p.cut ? counters[kTileTurn] : 0;
   // ---- a CTA's share of the call, in key tiles, and the works (parts of items) of each class ----
   if (threadIdx.x < kClasses) scratch->works[threadIdx.x] = 0;
   long long mine = 0;
@@ -538,10 +539,12 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         }
         if (!more) break;
       }
-      // The counters are zero again for the next launch.
+      // The counters are zero again for the next launch, and its turn is another. (Every CTA has
+      // read this launch's turn: it did so before its first item.)
       if (lane == 0 && atomicAdd(counters + kTileDone, 1) == (int)gridDim.x - 1) {
         counters[kTileNext] = 0;
         counters[kTileDone] = 0;
+        if (p.cut) counters[kTileTurn] = turn ^ 1;
       }
     } else if (warp == 0) {
       // ---------------- producer ----------------
@@ -776,6 +779,8 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       }
     } else {
       // ---------------- rows of an item's last V tile past the request's end ----------------
+      // (And the counters of the next launch's parts, which nothing here waits for.)
+      if (p.cut) clear_next_bank(counters, turn, blockIdx.x * 32 + lane, gridDim.x * 32);
       Reader reader;
       Item it;
       uint32_t step = 0, cleared[2] = {0, 0};
@@ -909,10 +914,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       if (quarter == 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->part_stored[x], part_count & 1));
         if (ok && lane == 0) {
-          int* counter = reinterpret_cast<int*>(p.work) + kTileParts + 2 * slot0 + x;
-          const bool last = atomicAdd(counter, 1) == parts - 1;
-          if (last) *counter = 0;  // as the next launch finds it
-          scratch->last[x] = last;
+          scratch->last[x] = atomicAdd(counters + tile_parts_at(turn, slot0, x), 1) == parts - 1;
           mbar_arrive(&bars->part_known[x]);
         }
       }
