@@ -414,8 +414,8 @@ tb_status tb_op_gemm_bias_act(tb_session* session, tb_stream* stream, const tb_t
  *     left as they were. A key row behind its sequence's end never reaches a result,
  *     whatever its bits. Inside a sequence a key row with a NaN or an infinity may reach
  *     rows that the causal mask hides it from.
- * Attributes of both attention operators: causal (0 or 1), scale (decimal string, > 0,
- * default 1/sqrt(D)), candidate. D <= 256. */
+ * Attributes of both attention operators: causal (0 or 1), scale (decimal string, > 0, held as
+ * a float: 1.4e-45 to 2.3e38; default 1/sqrt(D)), candidate. D <= 256. */
 
 /* "attention.varlen": Q [Tq, H, D], K/V [Tk, Hkv, D], request b's rows
  * cu_seqlens[b] .. cu_seqlens[b+1] of them; cu_seqlens [batch + 1], nondecreasing.

@@ -6,7 +6,10 @@ import subprocess
 import pytest
 
 import titan_rs_b200 as tb
+from titan_rs_b200 import _native as N
 from titan_rs_b200.kernel_abi import DType
+
+from test_serving_cpu import paged, varlen
 
 
 class UnlaunchedRuntime(tb.Runtime):
@@ -78,3 +81,12 @@ def test_no_launch_counts_parts_of_an_earlier_one(tmp_path):
                    text=True)
     done = subprocess.run([str(tmp_path / "banks")], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("call", [varlen, paged])
+def test_a_scale_that_is_no_float_is_refused(call):
+    for scale in ("1e-46", "1e-300", "2.4e38", "1e39", "1e300", "inf", "0", "1e-500"):
+        status, detail = call(attrs={"scale": scale})
+        assert status == N.TB_ERR_INVALID and "positive finite" in detail, (scale, detail)
+    for scale in ("1e-45", "1e-40", "2.3e38"):
+        assert call(attrs={"scale": scale}) == (N.TB_ERR_INVALID, "null session"), scale

@@ -99,3 +99,18 @@ def test_cut_requests_one_behind_another(session):
                 np.testing.assert_array_equal(b.outputs[0].to_numpy(runtime.stream), w)
     for b, w in zip(bound, want):
         np.testing.assert_array_equal(b.outputs[0].to_numpy(runtime.stream), w)
+
+
+@pytest.mark.parametrize("candidate", ["attention_tiles", "attention_rows", "attention_tokens"])
+def test_the_smallest_scales_give_means(session, rt, candidate):
+    """With a scale below the normal floats every visible key weighs the same, and a hidden one nothing."""
+    h, hk, d, page, dtype, lens, new = 4, 2, 64, 16, DType.BF16, [70, 5], [4, 3]
+    cu = prefix(new)
+    q, out = rows((7, h, d), dtype, 60), np.zeros((7, h, d), np.uint16)
+    k, v, table = make_cache(lens, page, hk, d, dtype, 61)
+    for scale in (1e-40, 1.4e-45):
+        name, got = run_paged(session, rt, q, k, v, table, lens, cu, out, dtype,
+                              {"scale": scale, "candidate": candidate, "max_query_len": 4})
+        assert name.startswith(candidate)
+        ref, mag = paged_reference(q, k, v, table, lens, cu, True, scale, as_f64(out))
+        assert_attention(got, ref, mag, dtype, 70, np.nanmax(np.abs(as_f64(v))))

@@ -33,8 +33,11 @@ tb_status parse_attrs(const tb_attr* attrs, uint32_t n, const char* op, bool pag
     } else if (strcmp(key, "scale") == 0) {
       char* end = nullptr;
       out->scale = attrs[i].str ? strtod(attrs[i].str, &end) : 0.0;
-      if (!attrs[i].str || end == attrs[i].str || *end != '\0' || !std::isfinite(out->scale) || !(out->scale > 0.0))
-        return contract(std::string(op) + " scale must be a positive finite number (decimal string)");
+      // (The kernels hold it, and its product with log2(e), as a float: a hidden score is -inf times
+      // it, which is no number where it is zero.)
+      const float held = (float)out->scale;
+      if (!attrs[i].str || end == attrs[i].str || *end != '\0' || !(held > 0.f) || !std::isfinite(held * 1.4426950408889634f))
+        return contract(std::string(op) + " scale must be a positive finite number of a float's range (decimal string)");
     } else if (paged && strcmp(key, "max_query_len") == 0) {
       if (attrs[i].str || attrs[i].value <= 0) return contract("attention.paged max_query_len must be a positive integer");
       out->max_query = (uint64_t)attrs[i].value;
