@@ -9,7 +9,7 @@ import titan_rs_b200 as tb
 from titan_rs_b200 import _native as N
 from titan_rs_b200.kernel_abi import DType
 
-from test_serving_cpu import paged, varlen
+from test_serving_cpu import execute, paged, tensor, varlen
 
 
 class UnlaunchedRuntime(tb.Runtime):
@@ -90,3 +90,19 @@ def test_a_scale_that_is_no_float_is_refused(call):
         assert status == N.TB_ERR_INVALID and "positive finite" in detail, (scale, detail)
     for scale in ("1e-45", "1e-40", "2.3e38"):
         assert call(attrs={"scale": scale}) == (N.TB_ERR_INVALID, "null session"), scale
+
+
+def test_append_refuses_rows_of_more_chunks_than_it_counts():
+    """A token's K and V rows in chunks of 16, 4 or 2 bytes: below 2^31 of them."""
+    def append(h, d, dtype, steps=None):
+        row = tensor(dtype, (1, h, d), steps)
+        cache = tensor(dtype, (1, 1, h, d), steps and (1,) + steps)
+        return execute("kv_cache.append", [row, row, tensor(N.TB_I32, (1,))], [cache, cache])
+
+    for h, d, dtype, steps in [(65535, 65535, N.TB_F32, None), (65535, 65535, N.TB_BF16, None),
+                               (65535, 32767, N.TB_BF16, None), (65535, 16385, N.TB_F32, None),
+                               (65535, 65528, N.TB_BF16, (1, 65529, 1))]:
+        status, detail = append(h, d, dtype, steps)
+        assert status == N.TB_ERR_INVALID and "i32 ABI" in detail, (h, d, detail)
+    for h, d, dtype in [(65535, 65532, N.TB_F32), (65535, 65528, N.TB_BF16), (65535, 16383, N.TB_BF16)]:
+        assert append(h, d, dtype) == (N.TB_ERR_INVALID, "null session"), (h, d)

@@ -17,6 +17,15 @@ bool same_rows(const tb_tensor* rows, const tb_tensor* cache) {
   return rows->rank == 3 && cache->rank == 4 && rows->shape[1] == cache->shape[2] && rows->shape[2] == cache->shape[3];
 }
 
+// The widest chunk (16, 4 or 2 bytes) that all of the or-ed addresses, steps and lengths are
+// multiples of.
+unsigned chunk_of(uint64_t bits) { return (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 2; }
+
+// Whether the kernel's 32-bit count of a token's chunks, of K and V, holds them.
+bool chunks_fit(uint64_t heads, uint64_t row_bytes, unsigned chunk) {
+  return 2 * heads * (row_bytes / chunk) + kAppendThreads <= 0x7fffffffull;
+}
+
 }  // namespace
 
 extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, const tb_tensor* k, const tb_tensor* v,
@@ -47,6 +56,12 @@ extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, con
     return contract("kv_cache.append requires a contiguous I32 slot_map [T]");
   if (!distinct_elements(k_cache) || !distinct_elements(v_cache))
     return contract("kv_cache.append requires caches whose elements do not overlap");
+  const int64_t size = (int64_t)dtype_size(dt);  // (a power of two, so it may be multiplied with the or-ed steps)
+  uint64_t steps = D;
+  for (int i = 0; i < 2; ++i) steps |= (uint64_t)(step_of(k, i) | step_of(v, i));
+  for (int i = 0; i < 3; ++i) steps |= (uint64_t)(step_of(k_cache, i) | step_of(v_cache, i));
+  steps *= (uint64_t)size;
+  if (!chunks_fit(H, D * size, chunk_of(steps))) return contract("kv_cache.append shape exceeds i32 ABI");
   if (!s) return set_error(TB_ERR_INVALID, "contract", "null session");
   tb_status rc;
   Stream* st = nullptr;
@@ -57,7 +72,6 @@ extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, con
       (rc = strided_buffer(s, k_cache, "kv_cache.append K cache", &bkc)) ||
       (rc = strided_buffer(s, v_cache, "kv_cache.append V cache", &bvc)) || (rc = activate(s)))
     return rc;
-  const int64_t size = (int64_t)dtype_size(dt);
   AppendParams p{};
   p.k = bk->ptr;
   p.v = bv->ptr;
@@ -78,11 +92,8 @@ extern "C" tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, con
   p.tokens = (int)T;
   p.heads = (int)H;
   p.page = (int)page;
-  // The widest chunk that every row start and the row length are multiples of.
-  uint64_t bits = p.k | p.v | p.k_cache | p.v_cache | (uint64_t)p.k_tok | (uint64_t)p.k_head | (uint64_t)p.v_tok |
-                  (uint64_t)p.v_head | (uint64_t)p.kc_page | (uint64_t)p.kc_tok | (uint64_t)p.kc_head |
-                  (uint64_t)p.vc_page | (uint64_t)p.vc_tok | (uint64_t)p.vc_head | (uint64_t)(D * size);
-  const unsigned chunk = (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 2;
+  const unsigned chunk = chunk_of(steps | p.k | p.v | p.k_cache | p.v_cache);
+  if (!chunks_fit(H, D * size, chunk)) return contract("kv_cache.append shape exceeds i32 ABI");
   const char* entry = chunk == 16 ? "kv_append_16" : chunk == 4 ? "kv_append_4" : "kv_append_2";
   p.chunks = (int)(D * size / chunk);
   CUfunction fn = nullptr;
