@@ -114,3 +114,19 @@ def test_the_smallest_scales_give_means(session, rt, candidate):
         assert name.startswith(candidate)
         ref, mag = paged_reference(q, k, v, table, lens, cu, True, scale, as_f64(out))
         assert_attention(got, ref, mag, dtype, 70, np.nanmax(np.abs(as_f64(v))))
+
+
+def test_a_request_past_max_query_len_takes_nothing_from_the_others(session, rt):
+    """max_query_len says too little for one request: its rows may be left, the others' may not."""
+    h, hk, d, page, dtype, bound = 32, 8, 128, 16, DType.BF16, 40
+    lens, new = [4000, 50, 300], [4000, bound, 33]
+    cu = prefix(new)
+    q = rows((int(cu[-1]), h, d), dtype, 70)
+    out = np.zeros((int(cu[-1]), h, d), np.uint16)
+    k, v, table = make_cache(lens, page, hk, d, dtype, 71)
+    name, got = run_paged(session, rt, q, k, v, table, lens, cu, out, dtype, {"max_query_len": bound})
+    assert name.startswith("attention_tiles")
+    at = cu[1]
+    ref, mag = paged_reference(q[at:], k, v, table[1:], lens[1:], cu[1:] - at, True, 1 / math.sqrt(d),
+                               as_f64(out[at:]))
+    assert_attention(got[at:], ref, mag, dtype, 300, np.nanmax(np.abs(as_f64(v))))

@@ -137,7 +137,7 @@ tb_status tmap_rows(CUtensorMap* map, uint32_t dtype, uint64_t base, int rank, c
 }
 
 // Tensor-core kernel for all requests but the token kernel's. `longest`: query rows of a request
-// at most.
+// at most, as the caller says.
 tb_status launch_tiles(Session* s, Stream* st, AttnCall* c, uint64_t longest) {
   AttnParams& p = c->p;
   const std::string suffix = std::string(c->dtype == TB_BF16 ? "bf16" : "f16") + "_d" + std::to_string(p.dim);
@@ -165,12 +165,14 @@ tb_status launch_tiles(Session* s, Stream* st, AttnCall* c, uint64_t longest) {
       (rc = tmap_rows(&mk, c->dtype, p.k, 4, kv_ext, k_steps, kv_box)) ||
       (rc = tmap_rows(&mv, c->dtype, p.v, 4, kv_ext, v_steps, kv_box)))
     return rc;
-  // Items (pairs of tiles x key heads) at most: every request may end inside a pair.
+  // Items (pairs of tiles x key heads) at most: every request may end inside a pair. What the caller
+  // says of the longest request only sizes the grid: a longer one has its items all the same,
+  // and takes none from the others.
   const uint64_t rows = 2ull * p.tile_tokens, tq = (uint64_t)p.tq, batch = (uint64_t)p.batch;
-  const uint64_t pairs = std::min(tq / rows + std::min(batch, tq), batch * ((longest + rows - 1) / rows));
-  uint64_t grid = pairs * (uint64_t)p.kv_heads;
-  if (grid > 0x3fffffffull) return contract("attention work list exceeds 2^30 items");
-  p.max_items = (int32_t)grid;
+  const uint64_t pairs = tq / rows + std::min(batch, tq);
+  if (pairs * (uint64_t)p.kv_heads > 0x3fffffffull) return contract("attention work list exceeds 2^30 items");
+  p.max_items = (int32_t)(pairs * (uint64_t)p.kv_heads);
+  uint64_t grid = std::min(pairs, batch * ((longest + rows - 1) / rows)) * (uint64_t)p.kv_heads;
   // One CTA an SM, drawing items until there are no more. The kernel may cut long requests
   // where two parts of the smallest size fit their keys.
   const uint64_t keys = p.table ? (uint64_t)p.width * p.page : (uint64_t)p.tk;
