@@ -132,6 +132,8 @@ tb_status tb_download(tb_session* session, tb_stream* stream, tb_buffer* src, vo
 /* DeviceSession::copy (titan-backend-cuda/src/lib.rs:1308-1320). */
 tb_status tb_copy(tb_session* session, tb_stream* stream, tb_buffer* dst, tb_buffer* src, size_t bytes,
                   tb_event** out);
+/* No counterpart in the reference. Zeroes the buffer's first `bytes`, in stream order. */
+tb_status tb_clear(tb_session* session, tb_stream* stream, tb_buffer* dst, size_t bytes, tb_event** out);
 
 /* Launch-argument kinds (LaunchArgKind, titan-types/src/lib.rs:80-88). */
 typedef enum tb_arg_kind { TB_ARG_BUFFER = 0, TB_ARG_SCALAR = 1, TB_ARG_SHAPE = 2 } tb_arg_kind;

@@ -105,6 +105,7 @@ CUresult cuCtxSynchronize() { return CUDA_SUCCESS; }
 CUresult cuMemAlloc(CUdeviceptr* p, size_t bytes) {
   void* m = aligned_alloc(256, (bytes + 255) & ~size_t(255));
   if (!m) return CUDA_ERROR_OUT_OF_MEMORY;
+  memset(m, 0xab, bytes);  // (what an earlier owner left)
   std::lock_guard<std::mutex> lock(mu);
   live[*p = (CUdeviceptr)m] = bytes;
   return CUDA_SUCCESS;

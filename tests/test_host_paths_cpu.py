@@ -73,3 +73,39 @@ session = tb.Session(0)  # (a fresh limit)
 requests = [plan(tb.Runtime(session), batch) for batch in (6500, 9000, 12000, 16000)]
 in_threads(*[lambda r=r: [r.enqueue() for _ in range(20)] for r in requests])
 """)
+
+
+def test_an_omitted_attention_output_begins_as_zeros(driver):
+    """Rows of no request are left as they were: in an output that the runtime makes they are zeros."""
+    host_driver.run(driver, """
+x = tb.TensorHandle.allocate(session, DType.BF16, (70, 4, 64))
+cu = tb.TensorHandle.allocate(session, DType.I32, (2,))
+assert x.to_numpy(rt.stream).any()  # (memory that something was in)
+cache = tb.TensorHandle.allocate(session, DType.BF16, (6, 16, 4, 64))
+table, lens = (tb.TensorHandle.allocate(session, DType.I32, s) for s in ((1, 6), (1,)))
+for request in (tb.OpRequest("attention.varlen", [x, x, x, cu], [spec_of(x)]),
+                tb.OpRequest("attention.paged", [x, cache, cache, table, lens, cu], [spec_of(x)])):
+    assert not rt.execute(request).outputs[0].to_numpy(rt.stream).any()
+    assert not rt.bind(request).outputs[0].to_numpy(rt.stream).any()
+    given = tb.TensorHandle.allocate(session, DType.BF16, (70, 4, 64))
+    assert rt.execute(request, output=given).outputs[0].to_numpy(rt.stream).all()
+""")
+
+
+def test_clear_checks_its_buffer(driver):
+    host_driver.run(driver, """
+b = session.allocate(64)
+def raised(call, text):
+    try:
+        call()
+    except tb.HalError as e:
+        assert text in str(e), e
+        return True
+assert raised(lambda: session.clear(rt.stream, b, 65), "exceeds allocation")
+other = tb.Session(0)
+assert raised(lambda: other.clear(other.create_stream(), b, 8), "foreign buffer")
+assert raised(lambda: other.clear(rt.stream, other.allocate(8), 8), "stream")
+x = tb.TensorHandle(session, b, DType.I32, (16,), (1,))
+session.wait(session.clear(rt.stream, b, 12))
+assert (x.to_numpy(rt.stream)[:3] == 0).all() and x.to_numpy(rt.stream)[3:].all()
+""")

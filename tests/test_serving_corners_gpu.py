@@ -130,3 +130,14 @@ def test_a_request_past_max_query_len_takes_nothing_from_the_others(session, rt)
     ref, mag = paged_reference(q[at:], k, v, table[1:], lens[1:], cu[1:] - at, True, 1 / math.sqrt(d),
                                as_f64(out[at:]))
     assert_attention(got[at:], ref, mag, dtype, 300, np.nanmax(np.abs(as_f64(v))))
+
+
+def test_rows_of_no_request_in_an_omitted_output_are_zeros(session, rt):
+    n, dtype = 500, DType.BF16
+    x = upload(session, rt.stream, rows((n, 4, 64), dtype, 80), dtype)
+    cu = ints(session, rt, [0, 40])
+    for _ in range(8):  # memory that another tensor was in
+        upload(session, rt.stream, np.full((n, 4, 64), 0x7FC1, np.uint16), dtype).buffer.release()
+        got = rt.execute(tb.OpRequest("attention.varlen", [x, x, x, cu], [spec_of(x)])).wait()
+        host = got.outputs[0].to_numpy(rt.stream)
+        assert host[:40].any() and not host[40:].any()

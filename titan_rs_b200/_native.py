@@ -105,6 +105,7 @@ _SIGNATURES = {
     "tb_upload": (_S, [_P, _P, _P, _P, _SZ, _PP]),
     "tb_download": (_S, [_P, _P, _P, _P, _SZ, _PP]),
     "tb_copy": (_S, [_P, _P, _P, _P, _SZ, _PP]),
+    "tb_clear": (_S, [_P, _P, _P, _SZ, _PP]),
     "tb_load": (_S, [_P, _P, _SZ, ctypes.c_char_p, ctypes.POINTER(LaunchMetadata), _PP]),
     "tb_kernel_release": (None, [_P]),
     "tb_builtin_cubin": (_S, [ctypes.c_char_p, _PP, ctypes.POINTER(_SZ)]),

@@ -806,6 +806,22 @@ tb_status tb_copy(tb_session* session, tb_stream* stream, tb_buffer* dst, tb_buf
   return record_event(s, st, nullptr, out);
 }
 
+tb_status tb_clear(tb_session* session, tb_stream* stream, tb_buffer* dst, size_t bytes, tb_event** out) {
+  Session* s = reinterpret_cast<Session*>(session);
+  if (!s) return set_error(TB_ERR_INVALID, "clear", "null session");
+  Stream* st = nullptr;
+  Buffer* bd = nullptr;
+  tb_status rc = check_stream(s, stream, &st);
+  if (rc) return rc;
+  rc = check_buffer(s, dst, &bd);
+  if (rc) return rc;
+  if (bytes > bd->bytes) return set_error(TB_ERR_INVALID, "clear", "transfer exceeds allocation");
+  rc = activate(s);
+  if (rc) return rc;
+  if (bytes) TB_CU("cuMemsetD8Async", driver()->cuMemsetD8Async(bd->ptr, 0, bytes, st->raw));
+  return record_event(s, st, nullptr, out);
+}
+
 tb_status tb_host_alloc(tb_session* session, size_t bytes, void** out) {
   Session* s = reinterpret_cast<Session*>(session);
   if (!s || !out) return set_error(TB_ERR_INVALID, "allocate", "null argument");

@@ -227,6 +227,12 @@ class Session:
         _check(N.lib().tb_copy(self.ptr, stream.ptr, dst.ptr, src.ptr, nbytes, ctypes.byref(h)))
         return Event(self, h.value)
 
+    def clear(self, stream: Stream, dst: Buffer, nbytes: int) -> Event:
+        """Zeroes the buffer's first `nbytes`, in stream order."""
+        h = _out()
+        _check(N.lib().tb_clear(self.ptr, stream.ptr, dst.ptr, nbytes, ctypes.byref(h)))
+        return Event(self, h.value)
+
     def load(self, artifact: bytes, abi_hash: str, metadata: dict) -> LoadedKernel:
         kinds = {"buffer": N.TB_ARG_BUFFER, "scalar": N.TB_ARG_SCALAR, "shape": N.TB_ARG_SHAPE}
         args = (N.LaunchArg * max(len(metadata["arguments"]), 1))()

@@ -185,6 +185,8 @@ _OUTPUTS = {"kv_cache.append": 2, "kv_cache.plan": 5}
 # Operators whose outputs may be strided. What the request says of such an output has to be what
 # the tensor passed for it is, since a wrong stride puts its rows elsewhere in the same memory.
 _STRIDED_OUTPUTS = {"attention.varlen", "attention.paged", "kv_cache.append", "kv_cache.plan"}
+# Operators that leave rows of their output as they were (those of no request).
+_LEAVES_ROWS = {"attention.varlen", "attention.paged"}
 _ARITY_MSG = {"softmax": "CUDA softmax requires exactly one input and one output",
               "gemm": "gemm requires exactly two rank-2 inputs",
               "scaled_dot_product_attention": "scaled dot-product attention requires exactly three rank-4 BHTD inputs",
@@ -218,7 +220,8 @@ class Runtime:
 
     def execute(self, request: OpRequest, output=None) -> ExecutionHandle:
         """Enqueues a request. `output`: the tensor to write, or the list of them for an operator
-        of several outputs; one output may be left out and is then allocated. An operator whose
+        of several outputs; one output may be left out and is then allocated (zeroed first, where
+        the operator leaves rows of it as they were). An operator whose
         outputs may be strided takes the strides of the tensor where the request's spec names none,
         and refuses a tensor that differs from its spec."""
         name = request.operator
@@ -254,7 +257,10 @@ class Runtime:
         if output is None and name not in _OUTPUTS:
             spec = request.outputs[0]
             try:
-                return request, [TensorHandle.allocate(self.session, spec.dtype, spec.shape)]
+                made = TensorHandle.allocate(self.session, spec.dtype, spec.shape)
+                if name in _LEAVES_ROWS:
+                    self.session.clear(self.stream, made.buffer, made.buffer.byte_len)
+                return request, [made]
             except HalError as e:
                 raise ExecutionError(name, "allocate", str(e), e.status) from e
         outputs = list(output) if isinstance(output, (list, tuple)) else [] if output is None else [output]
