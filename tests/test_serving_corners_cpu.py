@@ -2,6 +2,7 @@
 import pathlib
 import shutil
 import subprocess
+import sys
 
 import pytest
 
@@ -106,3 +107,25 @@ def test_append_refuses_rows_of_more_chunks_than_it_counts():
         assert status == N.TB_ERR_INVALID and "i32 ABI" in detail, (h, d, detail)
     for h, d, dtype in [(65535, 65532, N.TB_F32), (65535, 65528, N.TB_BF16), (65535, 16383, N.TB_BF16)]:
         assert append(h, d, dtype) == (N.TB_ERR_INVALID, "null session"), (h, d)
+
+
+NO_MEMORY = """
+import ctypes, resource
+from titan_rs_b200 import _native as N
+lib, handle = N.lib(), ctypes.c_void_p(0)
+t = N.Tensor()
+name = ctypes.create_string_buffer(b"x" * (1 << 28))
+# No room for another copy of the name.
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (1 << 26), resource.RLIM_INFINITY))
+print(lib.tb_execute_outputs(None, None, name, ctypes.byref(t), 1, ctypes.byref(t), 1, None, 0, None))
+print(lib.tb_execute(None, None, name, ctypes.byref(t), 1, ctypes.byref(t), None, 0, None))
+"""
+
+
+def test_the_router_returns_when_host_memory_runs_out():
+    """A C++ exception does not leave the C entries: they return a status."""
+    done = subprocess.run([sys.executable, "-c", NO_MEMORY], capture_output=True, text=True,
+                          cwd=pathlib.Path(__file__).resolve().parents[1])
+    assert done.returncode == 0, (done.returncode, done.stderr)
+    assert done.stdout.split() == [str(N.TB_ERR_OUT_OF_MEMORY)] * 2

@@ -14,7 +14,7 @@
 // capture, freed with the graph, shared with no other graph and no eager call. Graphs and
 // workspaces released while a stream is being captured are freed when the last capture ends.
 // A replay reads and writes the same device buffers the captured work named.
-#include "internal.hpp"
+#include "ops_common.hpp"
 
 namespace tb {
 
@@ -32,7 +32,7 @@ using namespace tb;
 
 extern "C" {
 
-tb_status tb_capture_begin(tb_session* session, tb_stream* stream) {
+tb_status tb_capture_begin(tb_session* session, tb_stream* stream) try {
   Session* s = reinterpret_cast<Session*>(session);
   if (!s) return set_error(TB_ERR_INVALID, "capture", "null session");
   Stream* st = nullptr;
@@ -44,9 +44,11 @@ tb_status tb_capture_begin(tb_session* session, tb_stream* stream) {
   st->capture = capture_id(st);
   if (st->capture) capture_began(s);
   return TB_OK;
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
-tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec** out) {
+tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec** out) try {
   Session* s = reinterpret_cast<Session*>(session);
   if (!s || !out) return set_error(TB_ERR_INVALID, "capture", "null argument");
   *out = nullptr;
@@ -57,9 +59,11 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
   if (rc) return rc;
   const DriverApi* d = driver();
   CUgraph graph = nullptr;
+  // What needs host memory comes before the capture's end, so that it can still be ended without.
   const unsigned long long id = st->capture;  // (an invalidated capture has lost its id in the driver)
-  st->capture = 0;
+  auto g = std::make_unique<GraphExec>();
   std::vector<CUdeviceptr> work = id ? take_captured_work(s, id) : std::vector<CUdeviceptr>();
+  st->capture = 0;
   const auto drop_work = [&] {
     retire_work(s, {nullptr, work, nullptr});
   };
@@ -86,17 +90,18 @@ tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec**
       return cu_error("cuEventCreate", e);
     }
   }
-  GraphExec* g = new GraphExec();
   g->session = s;
   g->done = done;
   g->exec = exec;
   g->work = std::move(work);
   s->refs.fetch_add(1);
-  *out = reinterpret_cast<tb_graph_exec*>(g);
+  *out = reinterpret_cast<tb_graph_exec*>(g.release());
   return TB_OK;
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
-tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_stream* stream) {
+tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_stream* stream) try {
   Session* s = reinterpret_cast<Session*>(session);
   GraphExec* g = reinterpret_cast<GraphExec*>(graph);
   if (!s || !g) return set_error(TB_ERR_INVALID, "launch", "null argument");
@@ -118,6 +123,8 @@ tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_str
   TB_CU("cuGraphLaunch", d->cuGraphLaunch(g->exec, st->raw));
   TB_CU("cuEventRecord", d->cuEventRecord(g->done, st->raw));
   return TB_OK;
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
 void tb_graph_exec_release(tb_graph_exec* graph) {
@@ -127,7 +134,7 @@ void tb_graph_exec_release(tb_graph_exec* graph) {
   const DriverApi* d = driver();
   if (d && g->exec) {
     d->cuCtxSetCurrent(s->context);
-    retire_work(s, {g->exec, g->work, g->done});
+    retire_work(s, {g->exec, std::move(g->work), g->done});
   }
   delete g;
   tb_session_release(reinterpret_cast<tb_session*>(s));

@@ -151,7 +151,7 @@ tb_status stream_workspace(Session* s, Stream* st, size_t bytes, CUdeviceptr* ou
 unsigned long long capture_id(Stream* st);
 // Frees a graph and workspaces when the work before `last` has ended: now, or, while a stream of
 // the session is being captured (which either would invalidate), when the last capture ends.
-void retire_work(Session* s, const RetiredWork& r);
+void retire_work(Session* s, RetiredWork r);
 void capture_began(Session* s);
 void capture_ended(Session* s);
 // Takes the workspaces of an ended capture out of the session's list.

@@ -63,7 +63,7 @@ extern "C" tb_status tb_execute(tb_session* session, tb_stream* stream, const ch
 extern "C" tb_status tb_execute_outputs(tb_session* session, tb_stream* stream, const char* op,
                                         const tb_tensor* inputs, uint32_t num_inputs, const tb_tensor* outputs,
                                         uint32_t num_outputs, const tb_attr* attrs, uint32_t num_attrs,
-                                        tb_event** out) {
+                                        tb_event** out) try {
   using tb::contract;
   if (!op) return contract("operator name is null");
   const Route* route = nullptr;
@@ -102,4 +102,6 @@ extern "C" tb_status tb_execute_outputs(tb_session* session, tb_stream* stream, 
       return tb_op_sdpa(session, stream, &q, &k, &v, &o, attrs, num_attrs, out);
     }
   }
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }

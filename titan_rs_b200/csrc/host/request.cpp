@@ -50,7 +50,7 @@ tb_status tb_request_create(tb_session* session, tb_stream* stream, const char* 
     Buffer* b = nullptr;
     if ((rc = check_buffer(s, t.buffer, &b))) return rc;
   }
-  Request* r = new Request();
+  auto r = std::make_unique<Request>();
   r->op = op;
   r->inputs.assign(inputs, inputs + num_inputs);
   r->outputs.assign(outputs, outputs + num_outputs);
@@ -67,18 +67,20 @@ tb_status tb_request_create(tb_session* session, tb_stream* stream, const char* 
   st->refs.fetch_add(1);
   for (const auto* list : {&r->inputs, &r->outputs})
     for (const tb_tensor& t : *list) tb_buffer_retain(t.buffer);
-  *out = reinterpret_cast<tb_request*>(r);
+  *out = reinterpret_cast<tb_request*>(r.release());
   return TB_OK;
 } catch (const std::exception& e) {
   return tb::caught(e);
 }
 
-tb_status tb_request_enqueue(const tb_request* request, tb_event** out) {
+tb_status tb_request_enqueue(const tb_request* request, tb_event** out) try {
   const Request* r = reinterpret_cast<const Request*>(request);
   if (!r) return contract("null request");
   return tb_execute_outputs(r->session, r->stream, r->op.c_str(), r->inputs.data(), (uint32_t)r->inputs.size(),
                             r->outputs.data(), (uint32_t)r->outputs.size(), r->attrs.data(), (uint32_t)r->attrs.size(),
                             out);
+} catch (const std::exception& e) {
+  return tb::caught(e);
 }
 
 void tb_request_release(tb_request* request) {

@@ -324,11 +324,14 @@ void free_work(const RetiredWork& r) {
 
 }  // namespace
 
-void retire_work(Session* s, const RetiredWork& r) {
+void retire_work(Session* s, RetiredWork r) {
   {
     std::lock_guard<std::mutex> lock(s->mu);
     if (s->captures > 0) {
-      s->retired.push_back(r);
+      try {
+        s->retired.push_back(std::move(r));
+      } catch (const std::bad_alloc&) {  // no room to remember it: the device memory stays taken
+      }
       return;
     }
   }
@@ -652,7 +655,10 @@ void tb_stream_release(tb_stream* stream) {
     }
     d->cuStreamDestroy_v2(x->raw);
     if (x->capture) {  // a capture that nothing ends any more
-      retire_work(s, {nullptr, take_captured_work(s, x->capture), nullptr});
+      try {
+        retire_work(s, {nullptr, take_captured_work(s, x->capture), nullptr});
+      } catch (const std::bad_alloc&) {  // (freed with the session)
+      }
       capture_ended(s);
     }
   }
