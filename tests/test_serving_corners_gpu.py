@@ -141,3 +141,43 @@ def test_rows_of_no_request_in_an_omitted_output_are_zeros(session, rt):
         got = rt.execute(tb.OpRequest("attention.varlen", [x, x, x, cu], [spec_of(x)])).wait()
         host = got.outputs[0].to_numpy(rt.stream)
         assert host[:40].any() and not host[40:].any()
+
+
+def halves_of_a_row(session, rt, op, candidate, group, n, gap, d=64):
+    """O of `group` heads over n f16 keys, of which the first scores `gap` above the others; v = 0 for it and
+    1 for them, so O is what the others weigh."""
+    dtype, page = DType.F16, 16
+    q = np.zeros((1, group, d), np.float16)
+    k, v = np.zeros((n, 1, d), np.float16), np.ones((n, 1, d), np.float16)
+    q[..., 0], k[0, 0, 0], v[0] = 1.0, gap, 0.0
+    attrs = {"scale": 1.0, "causal": False, "candidate": candidate}
+    spec = [tb.TensorSpec(dtype, q.shape)]
+    if op == "attention.varlen":
+        ins = [upload(session, rt.stream, x, dtype) for x in (q, k, v)] + [ints(session, rt, x) for x in ([0, 1], [0, n])]
+    else:
+        pages = -(-n // page)
+        caches = [np.zeros((pages * page, 1, d), np.float16) for _ in range(2)]
+        caches[0][:n], caches[1][:n] = k, v
+        ins = [upload(session, rt.stream, q, dtype)]
+        ins += [upload(session, rt.stream, c.reshape(pages, page, 1, d), dtype) for c in caches]
+        ins += [ints(session, rt, x) for x in (np.arange(pages)[None], [n], [0, 1])]
+        attrs["max_query_len"] = 1
+    got = rt.execute(tb.OpRequest(op, ins, spec, attrs)).wait()
+    assert got.candidate.startswith(candidate)
+    return got.outputs[0].to_numpy(rt.stream).astype(np.float64)
+
+
+@pytest.mark.parametrize("op,candidate,group", [("attention.varlen", "attention_tiles", 4),
+                                                ("attention.paged", "attention_tiles", 40),
+                                                ("attention.paged", "attention_tokens", 4),
+                                                ("attention.paged", "attention_tokens", 32),
+                                                ("attention.paged", "attention_rows", 4)])
+@pytest.mark.parametrize("n,gap", [(100000, 17.75), (131072, 14.0), (3000, 17.5)])
+def test_f16_keys_of_little_weight_count_together(session, rt, op, candidate, group, n, gap):
+    """Many keys that each weigh less than f16 holds next to 1: the weights are held 2^7 times as large,
+    so each is off by at most 2^-25 / 2^7 (or half a step, 2^-11 of it), and O by n times that. The
+    fp32 sums and ex2.approx are within 2^-11 of O, and O is rounded once (2^-11)."""
+    got = halves_of_a_row(session, rt, op, candidate, group, n, gap)
+    weight = math.exp(-gap)
+    want = (n - 1) * weight / (1 + (n - 1) * weight)
+    assert np.abs(got - want).max() <= 3 * 2.0 ** -11 * want + n * 2.0 ** -32 + 2.0 ** -25

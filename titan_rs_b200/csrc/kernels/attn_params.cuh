@@ -97,6 +97,13 @@ TB_BOTH constexpr int tile_smem_bytes(int dim) {
   return 7 * 128 * dim * 2 + kTileBarrierBytes + kTileScratchBytes + 1024;
 }
 
+// Probabilities are rounded to the values' type for the product with V: 2^(s - m), with a
+// reference m that may fall 8 behind the row's maximum. f16 has no more than 2^-24 next to 1, and
+// many keys of less would be lost together; so m is the maximum less 7 there. Probabilities and
+// their sum are 2^7 times as large (2^15 at most, below f16's 65504), the quotient is the same.
+// bf16 has fp32's exponents.
+constexpr float kF16WeightLog2 = 7.f;
+
 // The index arithmetic is shared by the kernels and a host test of it.
 #ifdef __CUDACC__
 // These kernels are launched with programmatic stream serialization (launch_overlapped):

@@ -213,8 +213,8 @@ __device__ __forceinline__ void scale_o(uint32_t o_tmem, float alpha) {
 
 // One key tile of one row's online softmax, as softmax_tile of the square kernel: the
 // reference maximum m moves only when the row's maximum grows by more than 2^8, so P stays
-// at or below 256. It starts at the lowest finite value, so a row (or a tile of it) without
-// a visible key adds exp2(-inf) = 0.
+// at or below 2^8 (in f16 2^15, see kF16WeightLog2). It starts at the lowest finite value, so a
+// row (or a tile of it) without a visible key adds exp2(-inf) = 0.
 template <typename T, int HD>
 __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, int valid, bool rescale, float scale2,
                                              float& m, float& l, uint64_t* p_half, uint64_t* p_full) {
@@ -251,9 +251,10 @@ __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, i
   mask_max_chunk(c2, BN, false, mx4);
   mask_max_chunk(c3, BN, false, mx4);
   const float mx = fmaxf(fmax3f(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale2;
-  const bool grow = mx > m + sdpa2::kLazyRescaleLog2;
+  constexpr float kBelow = __is_same(T, __half) ? kF16WeightLog2 : 0.f;  // of m below the maximum
+  const bool grow = mx > m + (sdpa2::kLazyRescaleLog2 + kBelow);
   if (__any_sync(0xffffffffu, grow)) {
-    const float m_new = grow ? mx : m;
+    const float m_new = grow ? mx - kBelow : m;
     const float alpha = exp2_mufu(m - m_new);
     l *= alpha;
     if (rescale) scale_o<HD>(o_tmem, alpha);

@@ -23,8 +23,9 @@
 //     warps help and fewer do not: 64 requests of 300-8192 keys (544 MB) 97 us against 108
 //     with two CTAs of three stages, 131 with three of 32-key tiles and 127 with one of 128-key
 //     tiles; four of 110-131 thousand (2.0 GB) 304 us, 6.6 TB/s, against 330.
-// Scores, statistics and O are fp32; P is rounded to the values' type for the second product
-// (at most 2^8: the reference maximum moves only when a row's maximum grows by more than 2^8).
+// Scores, statistics and O are fp32; P is rounded to the values' type for the second product (at
+// most 2^8, in f16 2^15: the reference maximum moves only when a row's maximum grows by more than
+// 2^8).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -371,6 +372,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
     // ---- softmax of the columns (query rows) over the warp's keys ----
     const int key = cur.tile * kTile + warp * 16 + (lane >> 2);
     uint32_t pf[NT][2];
+    constexpr float kBelow = __is_same(T, __half) ? kF16WeightLog2 : 0.f;  // of `top` below the maximum
     bool grow = false;
     float mx[NT][2];  // over the thread's own keys: the lanes only meet when a maximum grows
 #pragma unroll
@@ -381,7 +383,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mx[t][i] = fmaxf(s[t][i], s[t][i + 2]) * scale2;
-        grow |= mx[t][i] > top[t][i] + 8.f;
+        grow |= mx[t][i] > top[t][i] + (8.f + kBelow);
       }
     }
     if (__any_sync(0xffffffffu, grow)) {
@@ -390,7 +392,7 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float m = fmaxf(top[t][i], mx[t][i]);
+          float m = fmaxf(top[t][i], mx[t][i] - kBelow);
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
