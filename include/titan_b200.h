@@ -402,7 +402,8 @@ tb_status tb_op_gemm_bias_act(tb_session* session, tb_stream* stream, const tb_t
 
 /* No counterpart in the reference. Conventions of the four operators below:
  *   - BF16 or F16 values (kv_cache.append: F32 too), fp32 scores, softmax statistics and
- *     accumulation, one rounding of the output; I32 index tensors with contiguous rows.
+ *     accumulation. Two roundings to the values' type: of each probability, for its product
+ *     with V, and of the output. I32 index tensors with contiguous rows.
  *   - Value tensors may be strided: the innermost dimension contiguous, the others with any
  *     positive strides (a slice of a fused projection, a cache with heads before rows).
  *     Outputs' elements may not overlap each other or an input.
@@ -432,7 +433,8 @@ tb_status tb_op_attention_varlen(tb_session* session, tb_stream* stream, const t
  * tokens' own among them (written before by kv_cache.append). block_table [batch, width];
  * entries past a request's last page are not read. causal defaults to 1. Attribute
  * max_query_len: no request has more new tokens than this (default: Tq); a step of single
- * tokens gives 1 and launches less. Rows past the bound may be left as they were. */
+ * tokens gives 1 and takes the kernel for them. Rows of a request that is longer than it says
+ * may be left as they were; those of the others are written all the same. */
 tb_status tb_op_attention_paged(tb_session* session, tb_stream* stream, const tb_tensor* q, const tb_tensor* k_cache,
                                 const tb_tensor* v_cache, const tb_tensor* block_table, const tb_tensor* seq_lens,
                                 const tb_tensor* cu_seqlens_q, const tb_tensor* output, const tb_attr* attrs,
@@ -454,9 +456,9 @@ tb_status tb_op_kv_append(tb_session* session, tb_stream* stream, const tb_tenso
  * new_lens, [batch + 1]), slot_map (a slot for each packed token, -1 past the last one) and
  * status = {pages taken from the front of free_pages, requests refused}.
  * A request is refused when a length is negative or context + new passes 2^31 - 1, its pages
- * exceed the row, its tokens pass the end of slot_map, or free_pages ends before its pages (later requests that need pages
- * are then refused too): its seq_lens is its context, its slots are -1, its row is not
- * written. Up to 16384 requests. Attribute page_size (required). Outputs that share memory with
+ * exceed the row, its tokens pass the end of slot_map, or free_pages ends before its pages (all
+ * later requests are then refused too, those that need no page among them): its seq_lens is
+ * its context, its slots are -1, its row is not written. Up to 16384 requests. Attribute page_size (required). Outputs that share memory with
  * an input or each other are refused. */
 tb_status tb_op_kv_plan(tb_session* session, tb_stream* stream, const tb_tensor* context_lens,
                         const tb_tensor* new_lens, const tb_tensor* free_pages, const tb_tensor* block_table,

@@ -27,14 +27,16 @@
 //                finishes a tile's last part adds the parts up, in their order.
 // Bound by the chain of a tile's softmax and products: a step of the steady state takes about
 // 3,300 cycles, of which the tensor core works 2,176 and a tile's exponentials 2,048; an item
-// adds some 4,000 in which its rows are stored. Eight prompts of 4096 tokens (1.1 TFLOP under
-// the mask) take 976 us with 32 key heads and 935 with 8, 1.13 and 1.18 PFLOP/s against 1.04
-// of the square kernel on the same board.
+// adds some 4,000 in which its rows are stored. With the caches emptied in between, eight prompts
+// of 2900 to 4096 tokens, 32 heads (837 GFLOP under the mask) take 895 to 908 us over the boards
+// seen, 0.92 to 0.94 PFLOP/s; eight of 4096 (1.1 TFLOP) 1,121 us with 32 key heads and 1,074
+// with 8, 0.98 and 1.02 PFLOP/s.
 // Items of one to four steps are bound by the instruction caches, which the roles' code shares
 // and leaves behind: with the items' arithmetic in 32 bits and the mask, the copies of K and V,
 // the halves of P V and the rows' stores in loops, sixteen ragged prompts went from 125 to 114 us,
 // 24 of dimension 64 over other sequences' keys from 64 to 54, 128 of 256 tokens from 216
-// to 190. Built and not kept: two threads a row (sixteen softmax warps, 1,110 us where one
+// to 190 (launches in a row on one board; with the caches emptied in between, over several, the
+// kept form takes 119 to 122, 54.5 to 55 and 223). A thread spills 20 bytes. Built and not kept: two threads a row (sixteen softmax warps, 1,110 us where one
 // took 992: agreeing on the row's maximum costs more than the halves save), S read from tensor
 // memory a second time for the exponentials (less code, but 4 to 9% slower from four steps on),
 // items drawn earlier where they are short (up to 8% slower: the last ones are spread less

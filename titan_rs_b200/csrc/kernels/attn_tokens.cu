@@ -22,7 +22,10 @@
 //     chain (wait, first product, softmax, second product) and not the depth of the ring, so more
 //     warps help and fewer do not: 64 requests of 300-8192 keys (544 MB) 97 us against 108
 //     with two CTAs of three stages, 131 with three of 32-key tiles and 127 with one of 128-key
-//     tiles; four of 110-131 thousand (2.0 GB) 304 us, 6.6 TB/s, against 330.
+//     tiles; four of 110-131 thousand (2.0 GB) 304 us against 330 (launches in a row on one
+//     board). With the caches emptied in between, over the boards seen: 95 to 99 us (5.5 to 5.7
+//     TB/s) and 304 to 319 (6.3 to 6.6). A kernel that only reads as many bytes takes 79 and 276.
+//   - 17 to 32 query rows of dimension 128 take all 255 registers and spill 368 bytes a thread.
 // Scores, statistics and O are fp32; P is rounded to the values' type for the second product (at
 // most 2^8, in f16 2^15: the reference maximum moves only when a row's maximum grows by more than
 // 2^8).
