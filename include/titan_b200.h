@@ -414,9 +414,8 @@ tb_status tb_op_gemm_bias_act(tb_session* session, tb_stream* stream, const tb_t
  *   - With `causal` the mask is aligned at the sequences' ends: query row i of Lq sees the
  *     keys j <= Lk - Lq + i (tb_op_sdpa aligns at the start; the same when Lq == Lk).
  *   - A query row that sees no key gives zeros. Query rows behind cu_seqlens_q[batch] are
- *     left as they were. A key row behind its sequence's end never reaches a result,
- *     whatever its bits. Inside a sequence a key row with a NaN or an infinity may reach
- *     rows that the causal mask hides it from.
+ *     left as they were. Keys and values that a query row does not see, behind its sequence's
+ *     end or the causal mask, do not reach its result, whatever their bits.
  * Attributes of both attention operators: causal (0 or 1), scale (decimal string, > 0, held as
  * a float: 1.4e-45 to 2.3e38; default 1/sqrt(D)), candidate. D <= 256. */
 

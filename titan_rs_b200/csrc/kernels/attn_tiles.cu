@@ -15,10 +15,14 @@
 //                pages past the request's end, are given a coordinate outside the map, which
 //                the copy fills with zeros.
 //   warp 1       owns the tensor memory S_A | S_B | O_A | O_B; one lane issues the MMAs.
-//   warp 2       clears the rows of the last V tile that lie past the request's end (another
-//                request's, or whatever an unfinished page holds) between its copy and its
-//                use: their probabilities are 0, but 0 x NaN is not. Scores of such keys are
-//                replaced before use.
+//   warp 2       keeps what a row may not see out of P V, between a V tile's copy and its use: the
+//                probabilities are 0 there, but 0 x NaN is not. It clears the rows of the last tile
+//                that lie past the request's end (another request's, or whatever an unfinished page
+//                holds) or that none of the item's rows sees, and looks through those that only some see
+//                for infinities and NaNs. It clears these too, and the softmax warps add them to the
+//                rows that do see their keys when the item ends (sixteen ragged prompts 121.4 us
+//                without this, 122.2 with it; eight long ones 911 and 912; four short sequences 11.7
+//                and 12.0). Scores of hidden keys are replaced before use.
 //   warps 4..11  softmax, one row a thread, warps 4-7 tile A, 8-11 tile B.
 //   warp 3       items: persistent CTAs draw them from a counter. Requests with more key tiles than
 //                a CTA's share of the whole call are cut along the keys into parts, drawn first;
@@ -36,7 +40,8 @@
 // the halves of P V and the rows' stores in loops, sixteen ragged prompts went from 125 to 114 us,
 // 24 of dimension 64 over other sequences' keys from 64 to 54, 128 of 256 tokens from 216
 // to 190 (launches in a row on one board; with the caches emptied in between, over several, the
-// kept form takes 119 to 122, 54.5 to 55 and 223). A thread spills 20 bytes. Built and not kept: two threads a row (sixteen softmax warps, 1,110 us where one
+// kept form takes 119 to 122, 54.5 to 55 and 223). A thread spills up to 20 bytes. Built and not
+// kept: two threads a row (sixteen softmax warps, 1,110 us where one
 // took 992: agreeing on the row's maximum costs more than the halves save), S read from tensor
 // memory a second time for the exponentials (less code, but 4 to 9% slower from four steps on),
 // items drawn earlier where they are short (up to 8% slower: the last ones are spread less
@@ -79,7 +84,7 @@ struct Barriers {
   uint64_t p_half[2];                // per query tile: P of keys [0, 64) is in TMEM
   uint64_t p_full[2];                // per query tile: P of keys [64, 128) is in TMEM
   uint64_t o_full[2];                // per query tile: an item's last product is done
-  uint64_t v_raw[2];                 // per stage: a V tile whose rows past the end warp 2 clears
+  uint64_t v_raw[2];                 // per stage: a V tile that warp 2 looks at first
   uint64_t drain;
   uint64_t item_full[kSlots], item_empty[kSlots];
   uint64_t part_stored[2], part_known[2];  // per query tile: a part is in the workspace; whether it was the last one
@@ -89,15 +94,18 @@ struct Barriers {
 static_assert(sizeof(Barriers) <= kTileBarrierBytes, "barrier block overflows its reservation");
 
 // One item: two query tiles of one request and key head, and a range of key tiles.
-struct Item {
+struct alignas(16) Item {
   int n, n_a, n_b;       // key tiles of the part, and how many of them tiles A and B need; n < 0: no more items
   int lo;                // the first key tile
   int hk, b;             // key head, request
   int row, valid;        // tile A's first row of q, and rows from there to the request's end
   int base;              // local row i sees base + i keys (causal)
   int lk, k0;            // keys of the request, and its first row of k (packed)
-  int last_rows;         // rows of the last key tile if it runs past the request's end, else 0
-  int parts, part;       // parts that the item's keys are cut into, and which this is
+  int cut_from;          // the part's first key tile with keys that some row may not see (n: none)
+  short last_rows;       // rows of the last key tile if it runs past the request's end, else 0
+  bool special[2];       // whether one of the tiles from cut_from on that query tile x needs held an infinity or a
+                         // NaN (warp 2 says so before the tile's product, so it is settled when that ends)
+  short parts, part;     // parts that the item's keys are cut into, and which this is
   int slot, stride;      // slot of part 0, and the slots from one part to the next
 };
 
@@ -278,6 +286,90 @@ __device__ __forceinline__ void softmax_step(uint32_t s_tmem, uint32_t o_tmem, i
   tc_fence_before_sync();
   __syncwarp();
   if (lane == 0) mbar_arrive(p_full);
+}
+
+// Two 16-bit values each times zero, added to `sum`: zeros, or NaN where one is no finite number.
+template <typename T>
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t x, uint32_t sum) {
+  if constexpr (__is_same(T, __half)) {
+    const __half2 s = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2(), *reinterpret_cast<const __half2*>(&sum));
+    return *reinterpret_cast<const uint32_t*>(&s);
+  } else {
+    const __nv_bfloat162 s = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __nv_bfloat162(),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&sum));
+    return *reinterpret_cast<const uint32_t*>(&s);
+  }
+}
+
+template <typename T>
+constexpr uint32_t kExponent = __is_same(T, __half) ? 0x7c00u : 0x7f80u;  // all ones in an infinity or a NaN
+
+// Infinities and NaNs in rows [first, end) of a V tile become zeros. A warp's work.
+template <typename T>
+__device__ __noinline__ void clear_special(uint8_t* tile, int halves, int first, int end) {
+  for (int h = 0; h < halves; ++h) {
+    uint32_t* const at = reinterpret_cast<uint32_t*>(tile + h * 128 * 128);
+#pragma unroll 1
+    for (int i = first * 32 + lane_id(); i < end * 32; i += 32) {
+      uint32_t x = at[i];
+      if ((x & kExponent<T>) == kExponent<T>) x &= 0xffff0000u;
+      if ((x >> 16 & kExponent<T>) == kExponent<T>) x &= 0xffffu;
+      at[i] = x;
+    }
+  }
+}
+
+// Whether rows [first, end) of a V tile hold an infinity or a NaN. A warp's work, one load and four
+// instructions for 8 values, while the tile's softmax runs. (Four loads at a time: with one the
+// products wait for it, 948 us for long prompts where all rows are looked at, and 910 with four; with
+// eight the code costs the other roles more instruction fetches.)
+template <typename T, int kHalves>
+__device__ __forceinline__ bool has_special(const uint8_t* tile, int first, int end) {
+  uint32_t sum[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+  for (int h = 0; h < kHalves; ++h) {
+    const uint4* const at = reinterpret_cast<const uint4*>(tile + h * 128 * 128);
+#pragma unroll 4
+    for (int i = first * 8 + lane_id(); i < end * 8; i += 32) {
+      const uint4 x = at[i];
+      sum[0] = add_zero_times<T>(x.x, sum[0]);
+      sum[1] = add_zero_times<T>(x.y, sum[1]);
+      sum[2] = add_zero_times<T>(x.z, sum[2]);
+      sum[3] = add_zero_times<T>(x.w, sum[3]);
+    }
+  }
+  return __any_sync(0xffffffffu, ((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu) != 0);
+}
+
+// Adds the infinities and NaNs of V's rows [from, to) of the request, which clear_special took out, to
+// one row of O (a thread's). Called by all lanes of a warp; it is rare and reads V from memory.
+template <typename T, int HD>
+__device__ __noinline__ void add_special(const AttnParams& p, const Item& it, uint32_t o_tmem, int from, int to) {
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 16) {
+    uint32_t o[16];
+    tmem_ld_x16(o_tmem + c, o);
+    tmem_ld_wait();
+    reg_fence(o);
+#pragma unroll 1
+    for (int key = from; key < to; ++key) {
+      const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + it.hk * p.v_head + c;
+      if (p.table) {
+        const int id = page_of(p, it.b, key / p.page);
+        if (id < 0) continue;
+        v += id * p.v_page + key % p.page * p.v_tok;
+      } else {
+        v += (it.k0 + key) * p.v_tok;
+      }
+#pragma unroll
+      for (int d = 0; d < 16; ++d)
+        if ((v[d] & kExponent<T>) == kExponent<T>)
+          o[d] = __float_as_uint(__uint_as_float(o[d]) + (float)*reinterpret_cast<const T*>(v + d));
+    }
+    __syncwarp();
+    tmem_st_x16(o_tmem + c, o);
+  }
+  tmem_st_wait();
 }
 
 // A wait that sleeps between polls, for the warps beside the pipeline: they share issue slots
@@ -530,9 +622,11 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
           it.base = p.causal ? r.lk - r.lq + tok0 + 1 : r.lk;
           it.lk = r.lk;
           it.k0 = r.k0;
-          it.last_rows = it.n > 0 && hi == r.lk / BN + 1 ? r.lk % BN : 0;
-          it.parts = parts;
-          it.part = part;
+          it.last_rows = it.n > 0 && hi == r.lk / BN + 1 ? (short)(r.lk % BN) : (short)0;
+          // (The item's first row sees the fewest keys, `base` of them.)
+          it.cut_from = p.causal && it.base < r.lk ? min(max(max(it.base, 0) / BN - lo, 0), it.n) : it.n;
+          it.parts = (short)parts;
+          it.part = (short)part;
           it.slot = c == 0 ? w - part * heads : 0;
           it.stride = heads;
         }
@@ -642,7 +736,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         const int st = step & 1;
         ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars->kv_empty[st], ((step >> 1) & 1) ^ 1));
         if (!ok) break;
-        // A V tile with rows to clear goes to warp 2 first, which arrives on kv_full for the step.
+        // A V tile that warp 2 looks at goes to it first; it arrives on kv_full for the step.
         const bool raw = has_v && v_clear;
         if (lane == 0) {
           const uint32_t k_bytes = has_k ? S::kTileBytes : 0, v_bytes = has_v ? S::kTileBytes : 0;
@@ -657,9 +751,9 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         const int k_row = row_of(cur, cur.lo + j);
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-          if (!(t ? has_v : has_k)) continue;
-          load((t ? OFF_V : OFF_K) + st * S::kTileBytes, t ? &tmap_v : &tmap_k,
-               t && raw ? &bars->v_raw[st] : &bars->kv_full[st], t ? v_hk : cur.hk, t ? v_row : k_row, t ? v_page : w_now);
+          if (!(t ? has_k : has_v)) continue;
+          load((t ? OFF_K : OFF_V) + st * S::kTileBytes, t ? &tmap_k : &tmap_v,
+               !t && raw ? &bars->v_raw[st] : &bars->kv_full[st], t ? cur.hk : v_hk, t ? k_row : v_row, t ? w_now : v_page);
         }
         ++kv_issued[st];
         ++step;
@@ -668,7 +762,7 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         v_hk = cur.hk;
         v_row = row_of(cur, cur.lo + j);
         v_page = w_now;
-        v_clear = j + 1 == cur.n && cur.last_rows;
+        v_clear = j >= cur.cut_from || (j + 1 == cur.n && cur.last_rows);
         if (j == 0 && cur.n_b > 0) ok = load_q(cur, 1);
         w_now = w_next;
         w_next = w_after;
@@ -781,34 +875,47 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
         if (!mbar_wait(&bars->drain, 0)) report_status(status, kFailMma | 5);
       }
     } else {
-      // ---------------- rows of an item's last V tile past the request's end ----------------
+      // ---------------- what some row may not see of V ----------------
       // (And the counters of the next launch's parts, which nothing here waits for.)
       if (p.cut) clear_next_bank(counters, turn, blockIdx.x * 32 + lane, gridDim.x * 32);
       Reader reader;
       Item it;
       uint32_t step = 0, cleared[2] = {0, 0};
       bool owed = false;
-      while (reader.next<32, true>(bars, scratch, it) && it.n >= 0) {
+      bool ok = true;
+      while (ok) {
+        Item* const held = &scratch->items[reader.slot];  // (by the softmax warps, until the item ends)
+        if (!reader.next<32, true>(bars, scratch, it) || it.n < 0) break;
         if (it.n == 0 && owed) ++step;  // the step without scores
         owed = it.n > 0;
+        // (Of the item's last row. A tile that is looked at holds some key that it sees.)
+        const int last_seen = p.causal ? min(it.base + min(it.valid, 2 * p.tile_tokens) - 1, it.lk) : it.lk;
+        for (int j = min(it.cut_from, it.last_rows ? it.n - 1 : it.n); j < it.n; ++j) {
+          // Its V tile comes with the step behind its scores'.
+          const int st = (step + j + 1) & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_raw[st], (st ? cleared[1] : cleared[0]) & 1));
+          if (!ok) {
+            if (lane == 0) report_status(status, kFailClear | 1);
+            break;
+          }
+          ++(st ? cleared[1] : cleared[0]);
+          // Rows that all of the item's rows see, that some see, and that none does.
+          uint8_t* const tile = smem + OFF_V + st * S::kTileBytes;
+          const int start = (it.lo + j) * BN, some = max(it.base - start, 0), none = min(last_seen - start, BN);
+          for (int h = 0; h < S::kHalves; ++h) {
+            uint4* const at = reinterpret_cast<uint4*>(tile + h * S::kHalfBytes);
+            for (int i = none * 8 + lane; i < BN * 8; i += 32) at[i] = make_uint4(0, 0, 0, 0);
+          }
+          if (j >= it.cut_from && has_special<T, S::kHalves>(tile, some, none)) {
+            clear_special<T>(tile, S::kHalves, some, none);
+            if (lane == 0 && j < it.n_a) held->special[0] = true;
+            if (lane == 0 && j < it.n_b) held->special[1] = true;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->kv_full[st]);
+        }
         step += it.n;
-        if (it.last_rows == 0) continue;
-        // Its V tile comes with the step behind the item's last key tile.
-        const int st = step & 1;
-        if (!__all_sync(0xffffffffu, wait_idle(&bars->v_raw[st], (st ? cleared[1] : cleared[0]) & 1))) {
-          if (lane == 0) report_status(status, kFailClear | 1);
-          break;
-        }
-        ++(st ? cleared[1] : cleared[0]);
-        const int words = (BN - it.last_rows) * 8;  // 16-byte words of one half
-        for (int h = 0; h < S::kHalves; ++h) {
-          uint4* at =
-              reinterpret_cast<uint4*>(smem + OFF_V + st * S::kTileBytes + h * S::kHalfBytes + it.last_rows * 128);
-          for (int i = lane; i < words; i += 32) at[i] = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->kv_full[st]);
       }
     }
   } else {
@@ -860,6 +967,9 @@ __device__ __forceinline__ void attention_tiles(const AttnParams& p, const CUten
       }
       const bool in = used && i < it->valid;
       const int first = it->row, head0 = it->hk * group;
+      if (nx > 0 && it->special[x])
+        add_special<T, HD>(p, *it, o_tmem, max(it->base, (it->lo + it->cut_from) * BN),
+                           min(in ? seen : 0, (it->lo + nx) * BN));
       if (it->parts == 1) {
         reader.done(bars);
         const float inv = l == 0.f ? 0.f : 1.0f / l;

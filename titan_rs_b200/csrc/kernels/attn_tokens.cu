@@ -25,7 +25,7 @@
 //     tiles; four of 110-131 thousand (2.0 GB) 304 us against 330 (launches in a row on one
 //     board). With the caches emptied in between, over the boards seen: 95 to 99 us (5.5 to 5.7
 //     TB/s) and 304 to 319 (6.3 to 6.6). A kernel that only reads as many bytes takes 79 and 276.
-//   - 17 to 32 query rows of dimension 128 take all 255 registers and spill 368 bytes a thread.
+//   - 17 to 32 query rows of dimension 128 take all 255 registers and spill 316 bytes a thread.
 // Scores, statistics and O are fp32; P is rounded to the values' type for the second product (at
 // most 2^8, in f16 2^15: the reference maximum moves only when a row's maximum grows by more than
 // 2^8).
@@ -122,6 +122,54 @@ __device__ __forceinline__ void store_row4(T* to, const float4& o, float l) {
     reinterpret_cast<uint16_t*>(to)[2] = (uint16_t)hi;
     reinterpret_cast<uint16_t*>(to)[3] = (uint16_t)(hi >> 16);
   }
+}
+
+// The warp's 16 rows of V at `vs`, of keys from `key0` on: infinities and NaNs become zeros, and are
+// added to O of the query rows that see their keys. All lanes.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void take_special(uint32_t vs, int key0, const int (&seen)[NT][2],
+                                             float (&o)[NT][D / 16][4]) {
+  constexpr uint32_t kExponent = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+  constexpr int kChunks = D / 8;
+  const int lane = threadIdx.x & 31;
+  bool any = false;
+#pragma unroll 1
+  for (int i = lane; i < 16 * kChunks * 2; i += 32) {
+    uint2 x;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(vs + i * 8) : "memory");
+    any |= (x.x & kExponent) == kExponent || (x.x >> 16 & kExponent) == kExponent ||
+           (x.y & kExponent) == kExponent || (x.y >> 16 & kExponent) == kExponent;
+  }
+  if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll 1
+  for (int r = 0; r < 16; ++r) {
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // dimension k * 16 + h * 8 + lane / 4, as o holds them
+        uint16_t x;
+        asm volatile("ld.shared.u16 %0, [%1];"
+                     : "=h"(x) : "r"(vs + r * (D * 2) + (((k * 2 + h) ^ (r & 7)) << 4) + (lane >> 2) * 2) : "memory");
+        if ((x & kExponent) != kExponent) continue;
+        const float v = (float)*reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (key0 + r < seen[t][i]) o[t][k][2 * h + i] += v;
+      }
+    }
+  }
+  __syncwarp();
+#pragma unroll 1
+  for (int i = lane; i < 16 * kChunks * 4; i += 32) {
+    uint32_t x;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(vs + i * 4) : "memory");
+    if ((x & kExponent) == kExponent) x &= 0xffff0000u;
+    if ((x >> 16 & kExponent) == kExponent) x &= 0xffffu;
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(vs + i * 4), "r"(x) : "memory");
+  }
+  __syncwarp();
 }
 
 // Tiles of one (request, key head) pair; 0 for a request that is not this kernel's. A
@@ -422,6 +470,10 @@ __device__ __forceinline__ void attention_tokens(const AttnParams& p) {
       pf[t][1] = transpose8x8(Half<T>::pack(e[2], e[3]));
     }
     // ---- O^T += V^T P^T ----
+    // (Where some of the query rows may not see all of the warp's keys, a product of a hidden key's zero
+    // and an infinity or a NaN would reach them: such values are added by hand.)
+    if (cur.r.lq > 1 && p.causal && cur.tile * kTile + warp * 16 + 16 > cur.r.lk - cur.r.lq + 1)
+      take_special<T, D, NT>(vs, cur.tile * kTile + warp * 16, seen, o);
     {
       const int r = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
