@@ -213,8 +213,10 @@ uint64_t tb_stream_handle(const tb_stream* stream);
  * stream of the session with one launch, on the same device buffers. Host-staged
  * uploads/downloads, host waits and an operator's first use of per-stream scratch
  * (split-K, the persistent attention candidate: run it once first) cannot be
- * captured: tb_capture_end then returns the driver's error and no graph. A graph that holds
- * packed or paged attention is not launched into another capture (it owns their workspace). */
+ * captured: tb_capture_end then returns the driver's error and no graph. A graph of operators
+ * with scratch uses the captured stream's: replay it there, or while nothing else of the kind
+ * runs on that stream. A graph that holds packed or paged attention is not launched into
+ * another capture (it owns their workspace). */
 tb_status tb_capture_begin(tb_session* session, tb_stream* stream);
 tb_status tb_capture_end(tb_session* session, tb_stream* stream, tb_graph_exec** out);
 tb_status tb_graph_exec_launch(tb_session* session, tb_graph_exec* graph, tb_stream* stream);

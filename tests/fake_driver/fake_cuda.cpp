@@ -22,8 +22,16 @@ struct Function {
   int dynamic_limit;  // bytes; what is not asked for shares 48 KB with the static ones
 };
 
+// What a launch names: the kernel and its scratch memory, if it takes any.
+struct Launch {
+  std::string name;
+  CUdeviceptr scratch;
+};
+using Graph = std::vector<Launch>;
+
 std::mutex mu;
 std::map<CUdeviceptr, size_t> live;
+std::map<CUstream, Graph> capturing;
 std::vector<std::string> log;  // "launch NAME STREAM FIRST-POINTER", "error TEXT"
 std::atomic<uintptr_t> next_handle{0x1000};
 std::atomic<int> slow_ms{0};
@@ -37,7 +45,7 @@ void pause_if_slow() {
   if (const int ms = slow_ms.load()) std::this_thread::sleep_for(std::chrono::milliseconds(ms));
 }
 
-bool inside_live(CUdeviceptr p) {
+bool inside_live(CUdeviceptr p) {  // (with mu held)
   auto it = live.upper_bound(p);
   return it != live.begin() && p < (--it)->first + it->second;
 }
@@ -53,17 +61,20 @@ int scratch_parameter(const std::string& name) {
 
 int static_bytes(const std::string& name) { return name.rfind("kv_plan_", 0) == 0 ? 272 : 0; }
 
+void run(const Launch& l, CUstream stream) {
+  if (l.scratch && !inside_live(l.scratch)) log.push_back("error " + l.name + " launched on freed memory");
+  log.push_back("launch " + l.name + " " + std::to_string((uintptr_t)stream) + " " + std::to_string(l.scratch));
+}
+
 CUresult launch(const Function* f, unsigned shared, CUstream stream, void** params) {
   pause_if_slow();
   std::lock_guard<std::mutex> lock(mu);
   const int fixed = static_bytes(f->name);
   if ((int)shared > f->dynamic_limit && (int)shared + fixed > 48 * 1024) return CUDA_ERROR_INVALID_VALUE;
-  CUdeviceptr scratch = 0;
-  if (const int at = scratch_parameter(f->name); at >= 0) {
-    memcpy(&scratch, params[at], sizeof scratch);
-    if (!inside_live(scratch)) log.push_back("error " + f->name + " launched on freed memory");
-  }
-  log.push_back("launch " + f->name + " " + std::to_string((uintptr_t)stream) + " " + std::to_string(scratch));
+  Launch l{f->name, 0};
+  if (const int at = scratch_parameter(f->name); at >= 0) memcpy(&l.scratch, params[at], sizeof l.scratch);
+  if (auto it = capturing.find(stream); it != capturing.end()) it->second.push_back(l);
+  else run(l, stream);
   return CUDA_SUCCESS;
 }
 
@@ -141,18 +152,39 @@ CUresult cuStreamCreate(CUstream* s, unsigned) { return *s = handle<CUstream>(),
 CUresult cuStreamDestroy(CUstream) { return CUDA_SUCCESS; }
 CUresult cuStreamSynchronize(CUstream) { return CUDA_SUCCESS; }
 CUresult cuStreamWaitEvent(CUstream, CUevent, unsigned) { return CUDA_SUCCESS; }
-CUresult cuStreamBeginCapture(CUstream, CUstreamCaptureMode) { return CUDA_ERROR_NOT_SUPPORTED; }
-CUresult cuStreamIsCapturing(CUstream, CUstreamCaptureStatus* s) {
-  return *s = CU_STREAM_CAPTURE_STATUS_NONE, CUDA_SUCCESS;
+CUresult cuStreamBeginCapture(CUstream s, CUstreamCaptureMode) {
+  std::lock_guard<std::mutex> lock(mu);
+  return capturing.emplace(s, Graph()).second ? CUDA_SUCCESS : CUDA_ERROR_ILLEGAL_STATE;
 }
-CUresult cuStreamEndCapture(CUstream, CUgraph*) { return CUDA_ERROR_NOT_SUPPORTED; }
-CUresult cuStreamGetCaptureInfo_v2(CUstream, CUstreamCaptureStatus* s, cuuint64_t*, CUgraph*, const CUgraphNode**,
-                                   size_t*) {
-  return *s = CU_STREAM_CAPTURE_STATUS_NONE, CUDA_SUCCESS;
+CUresult cuStreamIsCapturing(CUstream stream, CUstreamCaptureStatus* s) {
+  std::lock_guard<std::mutex> lock(mu);
+  *s = capturing.count(stream) ? CU_STREAM_CAPTURE_STATUS_ACTIVE : CU_STREAM_CAPTURE_STATUS_NONE;
+  return CUDA_SUCCESS;
+}
+CUresult cuStreamEndCapture(CUstream s, CUgraph* g) {
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = capturing.find(s);
+  if (it == capturing.end()) return CUDA_ERROR_ILLEGAL_STATE;
+  *g = reinterpret_cast<CUgraph>(new Graph(it->second));
+  capturing.erase(it);
+  return CUDA_SUCCESS;
+}
+CUresult cuStreamGetCaptureInfo_v2(CUstream stream, CUstreamCaptureStatus* s, cuuint64_t* id, CUgraph*,
+                                   const CUgraphNode**, size_t*) {
+  cuStreamIsCapturing(stream, s);
+  if (id) *id = (cuuint64_t)(uintptr_t)stream;
+  return CUDA_SUCCESS;
 }
 CUresult cuThreadExchangeStreamCaptureMode(CUstreamCaptureMode*) { return CUDA_SUCCESS; }
-CUresult cuGraphInstantiateWithFlags(CUgraphExec*, CUgraph, unsigned long long) { return CUDA_ERROR_NOT_SUPPORTED; }
-CUresult cuGraphLaunch(CUgraphExec, CUstream) { return CUDA_ERROR_NOT_SUPPORTED; }
+CUresult cuGraphInstantiateWithFlags(CUgraphExec* e, CUgraph g, unsigned long long) {
+  *e = reinterpret_cast<CUgraphExec>(new Graph(*reinterpret_cast<Graph*>(g)));
+  return CUDA_SUCCESS;
+}
+CUresult cuGraphLaunch(CUgraphExec e, CUstream stream) {
+  std::lock_guard<std::mutex> lock(mu);
+  for (const Launch& l : *reinterpret_cast<Graph*>(e)) run(l, stream);
+  return CUDA_SUCCESS;
+}
 CUresult cuGraphExecDestroy(CUgraphExec) { return CUDA_SUCCESS; }
 CUresult cuGraphDestroy(CUgraph) { return CUDA_SUCCESS; }
 CUresult cuEventCreate(CUevent* e, unsigned) { return *e = handle<CUevent>(), CUDA_SUCCESS; }

@@ -109,3 +109,32 @@ x = tb.TensorHandle(session, b, DType.I32, (16,), (1,))
 session.wait(session.clear(rt.stream, b, 12))
 assert (x.to_numpy(rt.stream)[:3] == 0).all() and x.to_numpy(rt.stream)[3:].all()
 """)
+
+
+def test_a_graph_keeps_the_scratch_that_it_was_captured_on(driver):
+    """A larger operator on the stream, and the stream's release, leave a captured one's scratch memory."""
+    host_driver.run(driver, SCRATCH_USERS + """
+small, large = gemm(128, 128, 4096), gemm(256, 512, 4096)
+small.enqueue()
+session.capture_begin(rt.stream)
+small.enqueue()
+graph = session.capture_end(rt.stream)
+lines()
+large.enqueue()
+other = session.create_stream()
+for step in range(2):
+    graph.launch(other)
+    seen = lines()
+    assert [x.split()[1] for x in seen[-2:]] == ["gemm_bf16_tn_splitk", "splitk_reduce_bf16"], seen
+    assert not [x for x in seen if x.startswith("error")], seen
+    if step == 0:  # the larger one, captured too, outlives its stream
+        session.capture_begin(rt.stream)
+        large.enqueue()
+        second = session.capture_end(rt.stream)
+        rt.stream.release()
+        del small, large
+        import gc; gc.collect()
+second.launch(other)
+seen = lines()
+assert len(seen) == 2 and not [x for x in seen if x.startswith("error")], seen
+""")

@@ -53,6 +53,7 @@ struct Stream : RefCounted {
   // As the workspace below, it is taken and its kernels launched with `enqueue` held.
   CUdeviceptr scratch = 0;
   size_t scratch_bytes = 0;
+  bool scratch_captured = false;  // a graph names it
   // Workspace of the attention operators (zeroed when allocated; every launch leaves its counters
   // as the next one needs them, also one that gave up a wait). `enqueue` is held while an
   // operator takes it and launches, so that a second host thread on the stream cannot replace it
@@ -124,6 +125,7 @@ struct Session : RefCounted {
   std::unordered_map<CUfunction, int> shared_limit;  // dynamic shared memory that a kernel may be launched with
   std::unordered_set<void*> pinned;
   std::vector<CapturedWork> captured_work;  // of captures that have not ended
+  std::vector<CUdeviceptr> graph_scratch;  // streams' scratch that graphs name, replaced or left by its stream
   std::vector<RetiredWork> retired;  // to be freed when no stream is being captured any more
   int captures = 0;                  // streams being captured
   StatusWord status;

@@ -187,6 +187,8 @@ void session_destroy(Session* s) {
   }
   for (const CapturedWork& w : s->captured_work)
     if (d) d->cuMemFree_v2(w.ptr);
+  for (CUdeviceptr p : s->graph_scratch)
+    if (d) d->cuMemFree_v2(p);
   for (const RetiredWork& r : s->retired) {
     if (!d) break;
     if (r.exec) d->cuGraphExecDestroy(r.exec);  // (every stream has been waited for)
@@ -276,27 +278,43 @@ bool stream_capturing(Stream* st) {
   return driver()->cuStreamIsCapturing(st->raw, &status) == CUDA_SUCCESS && status != CU_STREAM_CAPTURE_STATUS_NONE;
 }
 
+// Frees the stream's scratch, or, where a graph names it, keeps it with the session (which the
+// graph holds).
+static void drop_scratch(Session* s, Stream* st) {
+  if (st->scratch_captured) {
+    std::lock_guard<std::mutex> lock(s->mu);
+    try {
+      s->graph_scratch.push_back(st->scratch);
+    } catch (const std::bad_alloc&) {  // no room to remember it: the device memory stays taken
+    }
+  } else {
+    driver()->cuMemFree_v2(st->scratch);
+  }
+  st->scratch = 0;
+  st->scratch_bytes = 0;
+  st->scratch_captured = false;
+}
+
 tb_status stream_scratch(Session* s, Stream* st, size_t bytes, CUdeviceptr* out) {
+  const bool capturing = stream_capturing(st);
   if (st->scratch_bytes >= bytes) {
+    st->scratch_captured |= capturing;
     *out = st->scratch;
     return TB_OK;
   }
-  if (stream_capturing(st))
+  if (capturing)
     return set_error(TB_ERR_INVALID, "capture",
                      "first use of the stream's scratch memory inside a graph capture: run the operator once before");
   const DriverApi* d = driver();
   if (st->scratch) {
     // Earlier kernels on this stream may still read the old scratch.
     TB_CU("cuStreamSynchronize", d->cuStreamSynchronize(st->raw));
-    d->cuMemFree_v2(st->scratch);
-    st->scratch = 0;
-    st->scratch_bytes = 0;
+    drop_scratch(s, st);
   }
   CUdeviceptr p = 0;
   TB_CU("allocate", d->cuMemAlloc_v2(&p, bytes));
   st->scratch = p;
   st->scratch_bytes = bytes;
-  (void)s;
   *out = p;
   return TB_OK;
 }
@@ -650,7 +668,7 @@ void tb_stream_release(tb_stream* stream) {
     d->cuCtxSetCurrent(s->context);
     if (x->scratch || x->work) {
       d->cuStreamSynchronize(x->raw);
-      if (x->scratch) d->cuMemFree_v2(x->scratch);
+      if (x->scratch) drop_scratch(s, x);
       if (x->work) retire_work(s, {nullptr, {x->work}, nullptr});
     }
     d->cuStreamDestroy_v2(x->raw);
