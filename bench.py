@@ -34,6 +34,7 @@ import json
 import math
 import os
 import pathlib
+import re
 import statistics
 import subprocess
 import sys
@@ -1186,20 +1187,20 @@ def main(argv=None) -> int:
 
 # DRAM bytes (dram__bytes_read.sum + dram__bytes_write.sum) of one full-size launch of
 # each kernel at N=1, from 1-pass ncu captures of bench.py. Each figure carries the
-# SHA-256 prefix of the kernel's sources (its .cu file, every shared .cuh and the tile
-# configuration header) at capture time; when the sources differ now, the figure
-# belongs to another build of the kernel and the bench prints null instead.
+# SHA-256 prefix of the kernel's sources (its .cu file and the headers beside it that it
+# includes) at capture time; when the sources differ now, the figure belongs to another
+# build of the kernel and the bench prints null instead.
 _TRAFFIC_CAPTURE = ("ncu --metrics dram__bytes_read.sum,dram__bytes_write.sum,gpu__time_duration.sum "
                     "--clock-control none -k regex:{kernel} -s 3 -c 1 python bench.py --op {op} --ops none "
                     "--steps 5 --warmup 3 --no-cpu-baseline --soak-ms 0")
 TRAFFIC_PER_LAUNCH: dict = {
-    "gemm_bf16_tn_2sm": {"read": 1044584704, "write": 126917888, "source_sha16": "a1c6ceac6de8b7b5",
+    "gemm_bf16_tn_2sm": {"read": 1044584704, "write": 126917888, "source_sha16": "121b69a3bacc52c8",
                          "capture": _TRAFFIC_CAPTURE.format(kernel="gemm_bf16_tn_2sm", op="gemm")},
-    "softmax_f32_warp32": {"read": 536921856, "write": 481277184, "source_sha16": "d9c1e674e4ee55f3",
+    "softmax_f32_warp32": {"read": 536921856, "write": 481277184, "source_sha16": "bc9e0cacf3cadd67",
                            "capture": _TRAFFIC_CAPTURE.format(kernel="softmax_f32_warp32", op="softmax")},
-    "sdpa_fwd_bf16_d128_pair": {"read": 817332224, "write": 250097664, "source_sha16": "634d5518b8f1f1b4",
+    "sdpa_fwd_bf16_d128_pair": {"read": 817332224, "write": 250097664, "source_sha16": "bce0fe12d3ef8e63",
                                 "capture": _TRAFFIC_CAPTURE.format(kernel="sdpa_fwd_bf16_d128_pair", op="sdpa")},
-    "conv2d_fprop_bf16_nhwc_2sm": {"read": 103998464, "write": 55198720, "source_sha16": "b42c3a7b52ea5292",
+    "conv2d_fprop_bf16_nhwc_2sm": {"read": 103998464, "write": 55198720, "source_sha16": "e456557465404678",
                                    "capture": _TRAFFIC_CAPTURE.format(kernel="conv2d_fprop_bf16_nhwc_2sm",
                                                                       op="conv2d")},
 }
@@ -1218,10 +1219,22 @@ def kernel_source_digest(kernel: str):
     if src is None:
         return None
     h = hashlib.sha256()
-    for path in [kdir / src] + sorted(kdir.glob("*.cuh")) + [kdir / "kernel_configs.h"]:
+    for path in included_sources(kdir / src):
         h.update(path.name.encode())
         h.update(path.read_bytes())
     return h.hexdigest()[:16]
+
+
+def included_sources(path: pathlib.Path) -> list:
+    """A kernel source and the headers of its folder that it includes, themselves or through others."""
+    found, waiting = [], [path]
+    while waiting:
+        path = waiting.pop()
+        if path in found or not path.exists():
+            continue
+        found.append(path)
+        waiting += [path.parent / name for name in re.findall(r'^\s*#\s*include\s*"([^"]+)"', path.read_text(), re.M)]
+    return [found[0]] + sorted(found[1:])
 
 
 def traffic_of(kernel: str, full_size_single_gpu: bool) -> dict:

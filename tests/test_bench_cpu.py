@@ -66,3 +66,23 @@ def test_traffic_figure_needs_the_captured_build():
     finally:
         bench.TRAFFIC_PER_LAUNCH.clear()
         bench.TRAFFIC_PER_LAUNCH.update(saved)
+
+
+def test_traffic_figures_belong_to_the_sources_beside_them(tmp_path, monkeypatch):
+    """A kernel's traffic figure follows its own sources and the headers it includes: those of the
+    default workloads are of the present ones, another kernel's header takes none away, and a change
+    in an included one does."""
+    import shutil
+    for kernel in bench.TRAFFIC_PER_LAUNCH:
+        assert bench.traffic_of(kernel, True)["traffic"], kernel
+    copy = tmp_path / "titan_rs_b200" / "csrc" / "kernels"
+    shutil.copytree(bench.ROOT / "titan_rs_b200" / "csrc" / "kernels", copy)
+    monkeypatch.setattr(bench, "ROOT", tmp_path)
+    (copy / "another.cuh").write_text("// not included\n")
+    (copy / "attn_params.cuh").write_text("// another kernel's\n")
+    for kernel in bench.TRAFFIC_PER_LAUNCH:
+        assert bench.traffic_of(kernel, True)["traffic"], kernel
+    with open(copy / "umma_pipeline_2sm.cuh", "a") as f:
+        f.write("// changed\n")
+    assert bench.traffic_of("gemm_bf16_tn_2sm", True)["traffic"] is None
+    assert bench.traffic_of("softmax_f32_warp32", True)["traffic"]

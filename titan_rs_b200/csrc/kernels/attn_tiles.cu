@@ -133,6 +133,12 @@ __device__ __forceinline__ bool elected() {
   return yes != 0;
 }
 
+// Adds to the bytes the current phase waits for, without arriving.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
+               : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <>
