@@ -136,6 +136,27 @@ def test_sdpa_bf16_is_bit_reproducible(session, rt):
     np.testing.assert_array_equal(a, b)
 
 
+@pytest.mark.parametrize("candidate", TC_CANDIDATES)
+@pytest.mark.parametrize("t", [64, 128, 200, 384])
+def test_sdpa_bf16_short_sequences_repeat_themselves(session, rt, candidate, t):
+    """Few key tiles and many CTAs, launched again and again: no warp reads O before its last products
+    are done, so every launch has the first one's bits, and those are right."""
+    b, h, d = 4, 64, 128
+    q, k, v = qkv_bf16(b, h, t, t, d, seed=80 + t)
+    ins = [upload(session, rt.stream, x, DType.BF16) for x in (q, k, v)]
+    out = tb.TensorHandle.allocate(session, DType.BF16, q.shape)
+    request = rt.bind(tb.OpRequest("scaled_dot_product_attention", ins, [tb.TensorSpec(DType.BF16, q.shape)],
+                                   {"causal": True, "candidate": candidate}), out)
+    request.enqueue()
+    first = out.to_numpy(rt.stream)
+    ids = np.arange(0, b * h * t, 7)
+    ref = oracle.sdpa_bf16_rows(q, k, v, b, h, t, t, d, True, ids)
+    assert max_rel_err(tb.bf16_bits_to_f32(first.reshape(-1, d)[ids]).reshape(-1, d), ref) <= BF16_TOL
+    for _ in range(25):
+        request.enqueue()
+        np.testing.assert_array_equal(out.to_numpy(rt.stream), first)
+
+
 def test_sdpa_default_candidate_and_unknown_candidate(session, rt):
     q, k, v = qkv_bf16(1, 1, 256, 256, 128, seed=9)
     assert run_sdpa(session, rt, q, k, v, True).candidate == "sdpa_fwd_bf16_d128_pair"

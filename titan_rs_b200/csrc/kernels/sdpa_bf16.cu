@@ -322,7 +322,10 @@ extern "C" __global__ void __launch_bounds__(THREADS, 1)
     }
     if (ok) {
       // ---------------- epilogue: O / l -> bf16 ----------------
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done, (n - 1) & 1));
+      // The last product's phase is told from the one two before it by parity alone, and the last
+      // scores only say that the product two before theirs is done: a warp ahead of the others
+      // waits for the product between as well.
+      ok = __all_sync(0xffffffffu, (n < 2 || mbar_wait(&bars->o_done, n & 1)) && mbar_wait(&bars->o_done, (n - 1) & 1));
       if (!ok) {
         if (lane == 0) report_status(status, kFailSoftmax | 4);
       } else {
